@@ -144,6 +144,80 @@ int natten_av_fwd(const natten_params_t* params, const void* attn, const void* v
 int natten_av_bwd(const natten_params_t* params, const void* attn, const void* v,
                   const void* dout, void* dattn, void* dv, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Around a decoder's cache (no counterpart in the reference): rotary positions, the append of new
+ * tokens to a paged cache and causal 1-D neighbourhood attention of new tokens over it.
+ *
+ *   q      [B, L, Hq,  D]  new tokens, padded to L a sequence; batch / token / head strides in elements
+ *   k, v   [B, L, Hkv, D]  the same
+ *   k_cache, v_cache  [pages, page_size, Hkv, D]  page / token / head strides, innermost axis contiguous
+ *   page_table [B, table_width]  int32 on the device: page of the sequence's tokens n * page_size ...;
+ *                                an entry outside [0, pages) is a page that is not there
+ *   cache_lens [B]         int32 on the device: tokens of the sequence, the new ones among them (attention: more
+ *                          than 2^30 are taken for 2^30)
+ *   seq_lens   [B]         int32 on the device, or NULL for L: new tokens of the sequence
+ * New token i of sequence b is at position cache_lens[b] - seq_lens[b] + i.  Nothing of this is read on the
+ * host: lengths are clamped to [0, L], and a position that is negative, past the table or on a page that is
+ * not there is neither read nor written.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct natten_rotary_params {
+    int32_t dtype;               /* NATTEN_F32 / F16 / BF16 / F64                                    */
+    int32_t batch, length, heads_q, heads_kv, dim;
+    int32_t rotary_dim;          /* leading channels of a head that are rotated (even, <= dim)      */
+    int32_t interleaved;         /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)           */
+    int32_t inverse;             /* rotate by the negative angle: the gradient                      */
+    int32_t reserved;
+    double magnitude;            /* what the rotated channels are multiplied by                     */
+    const double* frequencies;   /* device [rotary_dim / 2]: radians a position                     */
+    const int64_t* positions;    /* device, or NULL: token i is at position i                       */
+    int64_t position_stride[2];  /* batch, token                                                    */
+    int64_t q_stride[3];         /* batch, token, head strides (elements)                           */
+    int64_t k_stride[3];
+} natten_rotary_params_t;
+
+typedef struct natten_paged_params {
+    int32_t dtype;               /* attention: NATTEN_F32 / F16 / BF16; append: NATTEN_F64 as well  */
+    int32_t batch, length, heads_q, heads_kv, dim;
+    int32_t pages, page_size, table_width;
+    int32_t kernel;              /* attention: window, 0 = all of the past                          */
+    int32_t dilation;
+    int32_t rotary_dim;          /* append: as above, 0 = none                                      */
+    int32_t interleaved;
+    int32_t flags;               /* NATTEN_FLAG_*                                                   */
+    double scale;                /* attention: resolved logit scale                                 */
+    double magnitude;
+    const double* frequencies;
+    int64_t q_stride[3];         /* batch, token, head strides (elements)                           */
+    int64_t k_stride[3];         /* append only                                                     */
+    int64_t v_stride[3];
+    int64_t k_cache_stride[3];   /* page, token, head strides (elements)                            */
+    int64_t v_cache_stride[3];
+    int64_t table_stride;        /* between two sequences' rows of the page table                   */
+    const int32_t* page_table;
+    const int32_t* cache_lens;
+    const int32_t* seq_lens;
+} natten_paged_params_t;
+
+/* q_out = rotated q, k_out = rotated k (contiguous); k and k_out may both be NULL.  The gradient is the same
+ * call on the outputs' gradients with `inverse` set.                                                         */
+int natten_rotary(const natten_rotary_params_t* params, const void* q, const void* k, void* q_out, void* k_out,
+                  void* stream);
+
+/* k (rotated by the token's position where rotary_dim > 0) and v into the caches; with q also
+ * q_out [B, L, Hq, D] = rotated q (contiguous; rows past seq_lens are zero).  q and q_out may both be NULL.
+ * Two sequences that share a page they both write to race for it; no other slot of the cache is touched.      */
+int natten_paged_append(const natten_paged_params_t* params, const void* q, const void* k, const void* v,
+                        void* q_out, void* k_cache, void* v_cache, void* stream);
+
+/* out [B, L, Hq, D] = softmax(scale * q k^T) v over positions p, p - dilation, ..., p - (kernel - 1) * dilation
+ * of the query's own sequence (those that are there), lse [B, L, Hq] float (or NULL) its log-sum-exp.  Rows
+ * that see nothing and rows past seq_lens: out 0, lse -inf.  `workspace` holds the partial results of keys that
+ * several CTAs share, natten_paged_workspace_bytes(params) bytes (16-byte aligned); it needs no initial value
+ * and belongs to one call at a time.                                                                          */
+int natten_paged_fwd(const natten_paged_params_t* params, const void* q, const void* k_cache, const void* v_cache,
+                     void* out, void* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t natten_paged_workspace_bytes(const natten_paged_params_t* params);
+
 /* Diagnostics. */
 const char* natten_strerror(int code);
 int natten_abi_version(void);

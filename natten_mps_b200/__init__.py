@@ -10,11 +10,12 @@ from .version import __version__
 _LAZY = {
     **{n: "functional" for n in (
         "na1d", "na2d", "na3d", "na1d_qk", "na1d_av", "na2d_qk", "na2d_av", "na3d_qk", "na3d_av",
-        "na1d_varlen", "na2d_varlen", "na3d_varlen")},
+        "na1d_varlen", "na2d_varlen", "na3d_varlen", "na1d_rotary", "na1d_append", "na1d_paged")},
     "merge_attentions": "merge",
     "NeighborhoodAttention1D": "nn", "NeighborhoodAttention2D": "nn", "NeighborhoodAttention3D": "nn",
     "get_support_matrix": "support_matrix",
     "HostStep": "host_step",
+    "rotary_frequencies": "rotary", "PagedCache": "cache",
 }
 
 __all__ = sorted(list(_LAZY) + ["has_cuda", "get_backend", "set_backend", "__version__"])

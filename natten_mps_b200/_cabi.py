@@ -25,6 +25,7 @@ EXPORTS = (
     "natten_abi_version", "natten_last_path", "natten_launch_count", "natten_device_status",
     "natten_clear_status", "natten_status_async", "natten_host_status", "natten_debug_wait",
     "natten_fused_bwd_static", "natten_static_scratch_bytes",
+    "natten_rotary", "natten_paged_append", "natten_paged_fwd", "natten_paged_workspace_bytes",
 )
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float64: F64}
@@ -44,6 +45,34 @@ class Params(ctypes.Structure):
         ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3),
         ("v_stride", ctypes.c_int64 * 3),
         ("extents", ctypes.c_void_p),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``natten_rotary_params_t``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("length", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32), ("heads_kv", ctypes.c_int32), ("dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("reserved", ctypes.c_int32), ("magnitude", ctypes.c_double),
+        ("frequencies", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("position_stride", ctypes.c_int64 * 2),
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    """Mirror of ``natten_paged_params_t``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("length", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32), ("heads_kv", ctypes.c_int32), ("dim", ctypes.c_int32),
+        ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("kernel", ctypes.c_int32), ("dilation", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("scale", ctypes.c_double), ("magnitude", ctypes.c_double), ("frequencies", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("k_cache_stride", ctypes.c_int64 * 3), ("v_cache_stride", ctypes.c_int64 * 3),
+        ("table_stride", ctypes.c_int64), ("page_table", ctypes.c_void_p), ("cache_lens", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
     ]
 
 
@@ -74,6 +103,11 @@ def lib():
         L.natten_qk_rpb_bwd.argtypes = [pp] + [vp] * 7
         L.natten_av_fwd.argtypes = [pp] + [vp] * 4
         L.natten_av_bwd.argtypes = [pp] + [vp] * 6
+        L.natten_rotary.argtypes = [ctypes.POINTER(RotaryParams)] + [vp] * 5
+        L.natten_paged_append.argtypes = [ctypes.POINTER(PagedParams)] + [vp] * 7
+        L.natten_paged_fwd.argtypes = [ctypes.POINTER(PagedParams)] + [vp] * 6 + [ctypes.c_size_t, vp]
+        L.natten_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedParams)]
+        L.natten_paged_workspace_bytes.restype = ctypes.c_size_t
         L.natten_strerror.argtypes = [ctypes.c_int]
         L.natten_strerror.restype = ctypes.c_char_p
         L.natten_launch_count.restype = ctypes.c_ulonglong

@@ -15,6 +15,12 @@ They are thin compositions of four rank-generic ops that own the kernels:
     na_fused_bwd  -> (dq, dk, dv, d_extra_k, d_extra_v)
     na_qk / na_qk_bwd,  na_qk_rpb / na_qk_rpb_bwd,  na_av / na_av_bwd
 
+Beside them stand the operators around a decoder's cache, which the reference does not have:
+
+    na1d_rotary   -> (query, key)   rotary positions (its own backward pass, with ``inverse`` turned)
+    na1d_append   -> query          keys and values into a paged cache, in place; rotation on the way
+    na1d_paged    -> (out, lse)     causal neighbourhood attention of new tokens over a paged cache; no backward pass
+
 Schemas and ``Meta`` shape functions are here; the ``CUDA`` and autograd kernels are
 native (``csrc/torch_ops.cpp``).  Nothing is registered for other devices: calling an op
 with CPU tensors fails in the dispatcher instead of silently running something else.
@@ -122,6 +128,34 @@ def _na_qk_rpb_bwd_meta(dlogits, query, key, rpb_shape, kernel_size, dilation, s
 
 
 # ---------------------------------------------------------------------------
+# rotary positions, paged cache
+# ---------------------------------------------------------------------------
+LIB.define("na1d_rotary(Tensor query, Tensor key, Tensor frequencies, Tensor? positions, bool interleaved, "
+           "float magnitude, bool inverse) -> (Tensor, Tensor)")
+LIB.define("na1d_append(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor page_table, "
+           "Tensor cache_lens, Tensor? seq_lens, Tensor? query, Tensor? frequencies, bool interleaved, "
+           "float magnitude) -> Tensor")
+LIB.define("na1d_paged(Tensor query, Tensor key_cache, Tensor value_cache, Tensor page_table, Tensor cache_lens, "
+           "Tensor? seq_lens, int kernel_size, int dilation, float scale) -> (Tensor, Tensor)")
+
+
+@torch.library.impl(LIB, "na1d_rotary", "Meta")
+def _na1d_rotary_meta(query, key, frequencies, positions, interleaved, magnitude, inverse):
+    return query.new_empty(query.shape), key.new_empty(key.shape)
+
+
+@torch.library.impl(LIB, "na1d_append", "Meta")
+def _na1d_append_meta(key, value, key_cache, value_cache, page_table, cache_lens, seq_lens, query, frequencies,
+                      interleaved, magnitude):
+    return key.new_empty(0 if query is None else query.shape)
+
+
+@torch.library.impl(LIB, "na1d_paged", "Meta")
+def _na1d_paged_meta(query, key_cache, value_cache, page_table, cache_lens, seq_lens, kernel_size, dilation, scale):
+    return query.new_empty(query.shape), query.new_empty(query.shape[:-1], dtype=torch.float32)
+
+
+# ---------------------------------------------------------------------------
 # rank-specific names with the reference's schemas
 # ---------------------------------------------------------------------------
 def _define_rank_ops(rank: int) -> None:
@@ -167,7 +201,8 @@ def _define_rank_ops(rank: int) -> None:
 for _rank in (1, 2, 3):
     _define_rank_ops(_rank)
 
-OP_NAMES = ("na_fused", "na_fused_bwd", "na_qk", "na_qk_bwd", "na_qk_rpb", "na_qk_rpb_bwd", "na_av", "na_av_bwd") + tuple(
+OP_NAMES = ("na_fused", "na_fused_bwd", "na_qk", "na_qk_bwd", "na_qk_rpb", "na_qk_rpb_bwd", "na_av", "na_av_bwd",
+            "na1d_rotary", "na1d_append", "na1d_paged") + tuple(
     f"na{r}d_{s}" for r in (1, 2, 3) for s in ("qk", "av", "fwd", "varlen_fwd"))
 
 

@@ -1,0 +1,218 @@
+// Causal 1-D neighbourhood attention of new tokens over a paged cache: the geometry that its kernels share, and how they divide
+// the work.
+//
+// Dilation.  A query at position p sees p, p - d, p - 2d, ...: the positions of its residue modulo d.  So the new tokens of a
+// sequence fall into d classes (i mod d), and with t = (position - residue) / d each class is attention without dilation: query
+// u of the class stands at t = T0 + u and sees the keys t - K + 1 ... t.  Keys are fetched row by row through the page table
+// anyway, so a class's keys are as dense a tile as consecutive ones.
+//
+// Rows.  The query heads of a group share their keys: a row is (query u of the class, head g of the group), numbered u * G + g,
+// and a row tile is M consecutive rows, whatever G is.  A unit is (sequence, class, row tile, key/value head); its keys are the
+// union of its rows' windows, cut into tiles of `keys` keys from the first one on.
+//
+// Division of work.  The lengths are on the device, and differ.  Every CTA computes the number of key tiles of all units (the same
+// sums in every CTA), and takes the piece [c T / C, (c + 1) T / C) of their concatenation: equal shares, whatever the lengths are,
+// with no host read and no atomics.  A unit that lies inside one piece is written out directly.  Of one that several CTAs share,
+// each writes its unnormalised sum, maximum and row sum to the workspace (at most two units a CTA: one that its piece begins
+// inside of, one that it ends inside of), and a second kernel joins them, in the CTAs' order: results do not depend on timing.
+#pragma once
+#include "fast_div.cuh"
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace natten {
+namespace paged {
+
+constexpr int kAllOfThePast = 1 << 30;        // tokens of a sequence at most; as a window: no limit
+
+struct Args {
+    const void *q, *kc, *vc;
+    void* out;
+    float* lse;                              // may be null
+    unsigned char* ws;
+    const int *table, *cache_lens, *seq_lens;
+    int64_t table_stride, qs[3], ks[3], vs[3];
+    int B, L, Hq, Hkv, G, D;
+    int pages, page_size, table_width;
+    int K, dil;                              // window, at most kAllOfThePast
+    int M, keys, overhead, least;            // rows and keys of a tile; in key tiles: what beginning a unit costs, a CTA's least piece
+    int long_classes, tiles_long, tiles_short, per_seq, columns, ctas;
+    FastDiv by_page, by_group;
+    float scale_log2;                        // scale * log2(e)
+};
+
+// What a CTA tells the joining kernel: the unit that its piece ends inside of (its slot 2c + 1), the one that it begins inside of
+// (slot 2c), and whether it finishes that one.  -1: none.
+struct Shared { int tail, head, head_done, pad; };
+
+__host__ __device__ inline size_t shared_bytes(int ctas) { return (size_t)ctas * sizeof(Shared); }
+__host__ __device__ inline size_t slot_bytes(int M, int D) { return (size_t)M * (D + 2) * sizeof(float); }
+__device__ __forceinline__ float2* slot_sums(const Args& A, int slot)     // [M] maximum (of scale * log2(e) * score), row sum
+{
+    return reinterpret_cast<float2*>(A.ws + shared_bytes(A.ctas) + slot * slot_bytes(A.M, A.D));
+}
+__device__ __forceinline__ float* slot_out(const Args& A, int slot) { return reinterpret_cast<float*>(slot_sums(A, slot) + A.M); }
+
+struct Tile {                                // a row tile of a class of a sequence; the same for every key/value head
+    int b, cls, row0, rows;                  // rows: of the class, from row0 on, at most M
+    int fresh, t0, residue;                  // new tokens of the sequence; t of the class's first query
+    int lo, hi, n;                           // keys lo ... hi (t), in n tiles
+};
+
+__device__ __forceinline__ Tile tile_of(const Args& A, int column)
+{
+    Tile x;
+    x.b = column / A.per_seq;
+    int k = column - x.b * A.per_seq, queries = A.L / A.dil;
+    if (k < A.long_classes * A.tiles_long) {
+        x.cls = k / A.tiles_long;
+        k -= x.cls * A.tiles_long;
+        ++queries;
+    } else {
+        k -= A.long_classes * A.tiles_long;
+        const int c = k / A.tiles_short;
+        x.cls = A.long_classes + c;
+        k -= c * A.tiles_short;
+    }
+    x.row0 = k * A.M;
+    x.rows = min(A.M, queries * A.G - x.row0);
+    x.fresh = A.seq_lens ? min(max(A.seq_lens[x.b], 0), A.L) : A.L;
+    const int p = min(max(A.cache_lens[x.b], 0), kAllOfThePast) - x.fresh + x.cls;      // position of the class's first query
+    x.t0 = p >= 0 ? p / A.dil : -((-p + A.dil - 1) / A.dil);
+    x.residue = p - x.t0 * A.dil;
+    const int live = x.fresh > x.cls ? (x.fresh - x.cls + A.dil - 1) / A.dil : 0;
+    const int first = x.row0 / A.G, last = min((x.row0 + x.rows - 1) / A.G, live - 1);
+    const long long capacity = (long long)A.table_width * A.page_size;  // no position behind it exists
+    x.hi = x.t0 + last;
+    if (capacity <= x.residue) x.hi = -1;
+    else if (x.hi > (capacity - 1 - x.residue) / A.dil) x.hi = (int)((capacity - 1 - x.residue) / A.dil);
+    const int back = x.t0 + first - (A.K - 1);
+    x.lo = x.t0 + first > 0 && back > 0 ? back : 0;
+    x.n = last >= first && x.hi >= x.lo ? (x.hi - x.lo) / A.keys + 1 : 0;
+    return x;
+}
+
+// A CTA's piece, unit by unit.  `begin` is called by all `kThreads` threads; the rest is uniform arithmetic.
+struct Piece {
+    long long left;
+    int column, h, off;                      // where the piece goes on: unit (column, h), cost `off` into it
+    Tile tile;
+
+    // portion of the unit (column, h): key tiles [x0, x1).  n == 0: nothing to see, rows are to be cleared if `first`.
+    struct Portion { int h, x0, x1; bool work, whole, first; };
+
+    template <int kThreads> __device__ void begin(const Args& A, int cta, void* scratch)     // scratch: 32 + 4 long longs
+    {
+        long long* sums = static_cast<long long*>(scratch);
+        volatile long long* found = sums + 32;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        const int each = (A.columns + kThreads - 1) / kThreads;
+        const int c0 = min(A.columns, tid * each), c1 = min(A.columns, c0 + each);
+        long long mine = 0;
+        for (int c = c0; c < c1; ++c) mine += (long long)(tile_of(A, c).n + A.overhead) * A.Hkv;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        long long before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+        const long long from = before + upto - mine;
+        // no CTA gets less than `least`: every piece of a unit then has tiles, and a unit's CTAs are consecutive
+        const int n = (int)min((long long)A.ctas, max(total / A.least, 1ll));
+        const long long share = total / n, rest = total - share * n;       // total * cta / n without overflow
+        const long long start = cta < n ? share * cta + rest * cta / n : total, stop = cta < n ? share * (cta + 1) + rest * (cta + 1) / n : total;
+        if (start >= from && start < from + mine) {
+            long long at = start - from;
+            int c = c0;
+            for (;; ++c) {
+                const long long w = (long long)(tile_of(A, c).n + A.overhead) * A.Hkv;
+                if (at < w) break;
+                at -= w;
+            }
+            found[0] = c;
+            found[1] = at;
+        }
+        __syncthreads();
+        left = stop - start;
+        column = h = off = 0;
+        if (left > 0) {
+            column = (int)found[0];
+            tile = tile_of(A, column);
+            const int w = tile.n + A.overhead;
+            h = (int)(found[1] / w);
+            off = (int)(found[1] - (long long)h * w);
+        }
+    }
+    __device__ __forceinline__ bool more() const { return left > 0; }
+    __device__ __forceinline__ Portion portion(const Args& A) const
+    {
+        Portion p;
+        const int w = tile.n + A.overhead;
+        const int take = left < w - off ? (int)left : w - off;
+        p.h = h;
+        p.x0 = max(off - A.overhead, 0);
+        p.x1 = max(off + take - A.overhead, 0);
+        p.first = off == 0;
+        p.work = p.x1 > p.x0;
+        p.whole = p.work && p.x0 == 0 && p.x1 == tile.n;
+        return p;
+    }
+    __device__ __forceinline__ void advance(const Args& A)
+    {
+        const int w = tile.n + A.overhead;
+        const int take = left < w - off ? (int)left : w - off;
+        left -= take;
+        off += take;
+        if (off == w) {
+            off = 0;
+            if (++h == A.Hkv) {
+                h = 0;
+                if (++column < A.columns) tile = tile_of(A, column);
+                else left = 0;
+            }
+        }
+    }
+};
+
+// index of row r (< rows) of a tile in [B, L, Hq], and t of its query; false where there is no such query (a padding row)
+__device__ __forceinline__ bool row_of(const Args& A, const Tile& x, int h, int r, long long& index, int& t)
+{
+    const int row = x.row0 + r, u = A.by_group.div(row), g = row - u * A.G, i = x.cls + A.dil * u;
+    index = ((long long)x.b * A.L + i) * A.Hq + (long long)h * A.G + g;
+    t = x.t0 + u;
+    return i < x.fresh;
+}
+// offset of a row of q (elements)
+__device__ __forceinline__ long long query_offset(const Args& A, const Tile& x, int h, int r)
+{
+    const int row = x.row0 + r, u = A.by_group.div(row), g = row - u * A.G;
+    return x.b * A.qs[0] + (long long)(x.cls + A.dil * u) * A.qs[1] + (long long)(h * A.G + g) * A.qs[2];
+}
+// page and slot of key t of the tile's class: false where it is not there
+__device__ __forceinline__ bool locate(const Args& A, const Tile& x, int t, int& page, int& slot)
+{
+    if (t > x.hi) return false;              // hi is below the table's end
+    const int pos = x.residue + A.dil * t, n = A.by_page.div(pos);
+    slot = pos - n * A.page_size;
+    page = A.table[x.b * A.table_stride + n];
+    return page >= 0 && page < A.pages;
+}
+
+// Host side.  A kernel family says which tiles it would use (false: it does not cover the call); `plan` divides the call by
+// them.  `aligned`: every row of q and of the caches starts on a 16-byte boundary.
+struct Shape { int M, keys, overhead, least, ctas; };
+bool general_shape(int dtype, const Args& A, bool aligned, Shape& shape);
+int general_run(int dtype, const Args& A, bool aligned, cudaStream_t s);
+
+} // namespace paged
+} // namespace natten

@@ -363,6 +363,141 @@ std::tuple<Tensor, Tensor> av_bwd_cuda(const Tensor& dout_in, const Tensor& attn
     return {dattn, dv};
 }
 
+// ----------------------------------------------------------------------------- rotary positions, paged cache
+// int32 on the device, rows contiguous; wider integers are clamped (what does not fit is not there)
+Tensor as_index(const Tensor& t)
+{
+    const Tensor n = t.scalar_type() == at::kInt ? t : t.clamp(-1, 2147483647).to(at::kInt);
+    return n.dim() == 0 || n.stride(-1) == 1 ? n : n.contiguous();
+}
+void copy_strides(const Tensor& t, int64_t (&s)[3])      // [., ., heads, dim] with adjacent channels
+{
+    for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
+}
+
+std::tuple<Tensor, Tensor> rotary_cuda(const Tensor& q_in, const Tensor& k_in, const Tensor& freq_in, const OptTensor& positions,
+                                       bool interleaved, double magnitude, bool inverse)
+{
+    Tensor pos = positions.value_or(Tensor());
+    require_cuda({&q_in, &k_in, &freq_in, &pos}, q_in);
+    same_dtype(q_in, {&k_in});
+    TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && freq_in.dim() == 1, "natten_b200: na1d_rotary takes [B, L, H, D] tensors");
+    natten_rotary_params_t p{};
+    const c10::cuda::CUDAGuard guard(q_in.device());
+    const Tensor q = strided_input(q_in, 1, p.q_stride), k = strided_input(k_in, 1, p.k_stride), freq = as(freq_in, at::kDouble);
+    p.dtype = dtype_code(q.scalar_type());
+    p.batch = (int)q.size(0);
+    p.length = (int)q.size(1);
+    p.heads_q = (int)q.size(2);
+    p.heads_kv = (int)k.size(2);
+    p.dim = (int)q.size(3);
+    p.rotary_dim = 2 * (int)freq.numel();
+    p.interleaved = interleaved;
+    p.inverse = inverse;
+    p.magnitude = magnitude;
+    p.frequencies = freq.const_data_ptr<double>();
+    if (pos.defined()) {
+        if (pos.scalar_type() != at::kLong) pos = pos.to(at::kLong);
+        pos = pos.expand({q.size(0), q.size(1)});
+        p.positions = pos.const_data_ptr<int64_t>();
+        p.position_stride[0] = pos.stride(0);
+        p.position_stride[1] = pos.stride(1);
+    }
+    Tensor q_out = fresh(q.sizes(), q.scalar_type(), q), k_out = fresh(k.sizes(), q.scalar_type(), q);
+    poll_status(q);
+    check(natten_rotary(&p, ptr(q), ptr(k), out_ptr(q_out), out_ptr(k_out), stream_of(q)), "natten_rotary");
+    return {q_out, k_out};
+}
+
+// What append and attention have in common; the tensors that `p` points to are kept in `held`.
+void paged_params(natten_paged_params_t& p, const Tensor& like, int64_t heads_q, const Tensor& k_cache, const Tensor& v_cache,
+                  const Tensor& table, const Tensor& lens, const Tensor& fresh_lens, Tensor (&held)[3])
+{
+    TORCH_CHECK_VALUE(like.dim() == 4 && k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() && k_cache.size(3) == like.size(3) &&
+                          table.dim() == 2 && table.size(0) == like.size(0) && lens.dim() == 1 && lens.size(0) == like.size(0) &&
+                          (!fresh_lens.defined() || (fresh_lens.dim() == 1 && fresh_lens.size(0) == like.size(0))),
+                      "natten_b200: shapes of new tokens, caches, page table and lengths do not match");
+    for (const Tensor* c : {&k_cache, &v_cache})
+        TORCH_CHECK_VALUE(c->size(3) == 1 || c->stride(3) == 1 || c->numel() == 0, "natten_b200: a cache's channels must be adjacent in memory");
+    TORCH_CHECK_VALUE(k_cache.size(0) <= 2147483647 && k_cache.size(1) <= 2147483647, "natten_b200: too many pages");
+    held[0] = as_index(table);
+    held[1] = as_index(lens);
+    if (fresh_lens.defined()) held[2] = as_index(fresh_lens);
+    p.dtype = dtype_code(like.scalar_type());
+    p.batch = (int)like.size(0);
+    p.length = (int)like.size(1);
+    p.heads_q = (int)heads_q;
+    p.heads_kv = (int)k_cache.size(2);
+    p.dim = (int)like.size(3);
+    p.pages = (int)k_cache.size(0);
+    p.page_size = (int)k_cache.size(1);
+    p.table_width = (int)table.size(1);
+    copy_strides(k_cache, p.k_cache_stride);
+    copy_strides(v_cache, p.v_cache_stride);
+    p.table_stride = held[0].stride(0);
+    p.page_table = held[0].const_data_ptr<int32_t>();
+    p.cache_lens = held[1].const_data_ptr<int32_t>();
+    p.seq_lens = held[2].defined() ? held[2].const_data_ptr<int32_t>() : nullptr;
+    p.flags = g_flags.load(std::memory_order_relaxed);
+}
+
+// the rotated query; an empty tensor where there is none
+Tensor append_cuda(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                   const Tensor& lens, const OptTensor& seq_lens, const OptTensor& query, const OptTensor& frequencies, bool interleaved,
+                   double magnitude)
+{
+    const Tensor q_in = query.value_or(Tensor()), freq_in = frequencies.value_or(Tensor()), fresh_lens = seq_lens.value_or(Tensor());
+    require_cuda({&k_in, &v_in, &k_cache, &v_cache, &table, &lens, &fresh_lens, &q_in, &freq_in}, k_in);
+    same_dtype(k_in, {&v_in, &k_cache, &v_cache, &q_in});
+    const c10::cuda::CUDAGuard guard(k_in.device());
+    natten_paged_params_t p{};
+    Tensor held[3], q, q_out, freq;
+    paged_params(p, k_in, q_in.defined() ? q_in.size(2) : 1, k_cache, v_cache, table, lens, fresh_lens, held);
+    TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.size(2) == k_cache.size(2), "natten_b200: key, value and cache do not match");
+    const Tensor k = strided_input(k_in, 1, p.k_stride), v = strided_input(v_in, 1, p.v_stride);
+    if (q_in.defined()) {
+        q = strided_input(q_in, 1, p.q_stride);
+        q_out = fresh(q.sizes(), q.scalar_type(), q);
+    }
+    if (freq_in.defined()) {
+        freq = as(freq_in, at::kDouble);
+        p.rotary_dim = 2 * (int)freq.numel();
+        p.frequencies = freq.const_data_ptr<double>();
+    }
+    p.interleaved = interleaved;
+    p.magnitude = magnitude;
+    poll_status(k);
+    check(natten_paged_append(&p, ptr(q), ptr(k), ptr(v), out_ptr(q_out), k_cache.mutable_data_ptr(), v_cache.mutable_data_ptr(),
+                              stream_of(k)),
+          "natten_paged_append");
+    return q_out.defined() ? q_out : fresh({0}, k.scalar_type(), k);
+}
+
+std::tuple<Tensor, Tensor> paged_cuda(const Tensor& q_in, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                                      const Tensor& lens, const OptTensor& seq_lens, int64_t kernel, int64_t dilation, double scale)
+{
+    const Tensor fresh_lens = seq_lens.value_or(Tensor());
+    require_cuda({&q_in, &k_cache, &v_cache, &table, &lens, &fresh_lens}, q_in);
+    same_dtype(q_in, {&k_cache, &v_cache});
+    TORCH_CHECK_VALUE(kernel >= 0 && dilation >= 1 && dilation <= 2147483647, "natten_b200: kernel_size and dilation must be positive");
+    const c10::cuda::CUDAGuard guard(q_in.device());
+    natten_paged_params_t p{};
+    Tensor held[3];
+    paged_params(p, q_in, q_in.size(2), k_cache, v_cache, table, lens, fresh_lens, held);
+    const Tensor q = strided_input(q_in, 1, p.q_stride);
+    p.kernel = (int)std::min<int64_t>(kernel, 2147483647);
+    p.dilation = (int)dilation;
+    p.scale = scale;
+    Tensor out = fresh(q.sizes(), q.scalar_type(), q), lse = fresh(q.sizes().slice(0, 3), at::kFloat, q);
+    const size_t ws_bytes = std::max<size_t>(natten_paged_workspace_bytes(&p), 256);
+    Tensor ws = fresh({(int64_t)ws_bytes}, at::kByte, q);
+    poll_status(q);
+    check(natten_paged_fwd(&p, ptr(q), k_cache.const_data_ptr(), v_cache.const_data_ptr(), out_ptr(out), out_ptr(lse), out_ptr(ws), ws_bytes,
+                           stream_of(q)),
+          "natten_paged_fwd");
+    return {out, lse};
+}
+
 // ----------------------------------------------------------------------------- dispatcher handles
 template <typename Sig> auto handle(const char* name)
 {
@@ -390,6 +525,25 @@ Tensor call_qk_rpb(const Tensor& q, const Tensor& k, const Tensor& rpb, IntArray
 {
     static const auto op = handle<decltype(qk_rpb_cuda)>("natten_b200::na_qk_rpb");
     return op.call(q, k, rpb, ks, dil, scale);
+}
+
+std::tuple<Tensor, Tensor> call_rotary(const Tensor& q, const Tensor& k, const Tensor& freq, const OptTensor& positions, bool interleaved,
+                                       double magnitude, bool inverse)
+{
+    static const auto op = handle<decltype(rotary_cuda)>("natten_b200::na1d_rotary");
+    return op.call(q, k, freq, positions, interleaved, magnitude, inverse);
+}
+Tensor call_append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lens,
+                   const OptTensor& seq_lens, const OptTensor& query, const OptTensor& freq, bool interleaved, double magnitude)
+{
+    static const auto op = handle<decltype(append_cuda)>("natten_b200::na1d_append");
+    return op.call(k, v, k_cache, v_cache, table, lens, seq_lens, query, freq, interleaved, magnitude);
+}
+std::tuple<Tensor, Tensor> call_paged(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lens,
+                                      const OptTensor& seq_lens, int64_t kernel, int64_t dilation, double scale)
+{
+    static const auto op = handle<decltype(paged_cuda)>("natten_b200::na1d_paged");
+    return op.call(q, k_cache, v_cache, table, lens, seq_lens, kernel, dilation, scale);
 }
 
 // ----------------------------------------------------------------------------- autograd
@@ -557,6 +711,74 @@ Tensor qk_rpb_autograd(const Tensor& q, const Tensor& k, const Tensor& rpb, IntA
         return call_qk_rpb(q, k, rpb, ks, dil, scale);
     }
     return QkRpbFn::apply(q, k, rpb, ks, dil, scale);
+}
+
+// Rotation is linear and its transpose is the rotation by the negative angle: the backward pass is the operator itself (and so
+// has a gradient of its own).
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& freq, const OptTensor& positions,
+                                 bool interleaved, double magnitude, bool inverse)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [qr, kr] = call_rotary(q, k, freq, positions, interleaved, magnitude, inverse);
+        ctx->saved_data["f"] = std::vector<int64_t>{interleaved, inverse};
+        ctx->saved_data["s"] = magnitude;
+        ctx->save_for_backward({freq, positions.value_or(Tensor())});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["q"] = q.sizes().vec();
+        ctx->saved_data["k"] = k.sizes().vec();
+        return {qr, kr};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        const auto f = ctx->saved_data.at("f").toIntVector();
+        Tensor dq = grads[0], dk = grads[1];
+        if (!dq.defined() && !dk.defined()) return {{}, {}, {}, {}, {}, {}, {}};
+        // one launch for both; an output that nothing was made of has the gradient zero
+        if (!dq.defined()) dq = at::zeros(ctx->saved_data.at("q").toIntVector(), dk.options());
+        if (!dk.defined()) dk = at::zeros(ctx->saved_data.at("k").toIntVector(), dq.options());
+        auto [gq, gk] = call_rotary(dq, dk, s[0], s[1].defined() ? OptTensor(s[1]) : OptTensor(), f[0] != 0, *saved_scale(ctx), f[1] == 0);
+        return {gq, gk, {}, {}, {}, {}, {}};
+    }
+};
+std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& freq, const OptTensor& positions,
+                                           bool interleaved, double magnitude, bool inverse)
+{
+    TORCH_CHECK_VALUE(!wants_grad({&freq}), "natten_b200: the frequencies of na1d_rotary have no gradient");
+    if (!wants_grad({&q, &k})) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return call_rotary(q, k, freq, positions, interleaved, magnitude, inverse);
+    }
+    const variable_list r = RotaryFn::apply(q, k, freq, positions, interleaved, magnitude, inverse);
+    return {r[0], r[1]};
+}
+
+void no_backward(std::initializer_list<const Tensor*> tensors, const char* what)
+{
+    TORCH_CHECK(!wants_grad(tensors), "natten_b200: ", what, " has no backward pass (it serves a cache); call it under torch.no_grad() "
+                "or with detached tensors");
+}
+Tensor append_autograd(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                       const Tensor& lens, const OptTensor& seq_lens, const OptTensor& query, const OptTensor& freq, bool interleaved,
+                       double magnitude)
+{
+    no_backward({&k, &v, &k_cache, &v_cache, opt_ptr(query), opt_ptr(freq)}, "na1d_append");
+    Tensor out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = call_append(k, v, k_cache, v_cache, table, lens, seq_lens, query, freq, interleaved, magnitude);
+    }
+    for (const Tensor* c : {&k_cache, &v_cache})
+        if (!c->is_inference()) c->unsafeGetTensorImpl()->bump_version();       // written in place
+    return out;
+}
+std::tuple<Tensor, Tensor> paged_autograd(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                                          const Tensor& lens, const OptTensor& seq_lens, int64_t kernel, int64_t dilation, double scale)
+{
+    no_backward({&q, &k_cache, &v_cache}, "na1d_paged");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_paged(q, k_cache, v_cache, table, lens, seq_lens, kernel, dilation, scale);
 }
 
 // The whole module, projections included, as one node of the autograd graph.  Built from the separate operators a training
@@ -983,6 +1205,129 @@ PyObject* py_av(PyObject*, PyObject* const* args, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+bool boolean(PyObject* o, bool& out)
+{
+    if (o != Py_True && o != Py_False) return false;
+    out = o == Py_True;
+    return true;
+}
+PyObject* pair_of(Tensor a, Tensor b)
+{
+    PyObject* both = PyTuple_New(2);
+    if (!both) return nullptr;
+    PyTuple_SET_ITEM(both, 0, wrap(std::move(a)));
+    PyTuple_SET_ITEM(both, 1, wrap(std::move(b)));
+    return both;
+}
+bool whole_numbers(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+// None, or frequencies that fit a head of `dim` channels
+bool turn(PyObject* o, int64_t dim, OptTensor& freq)
+{
+    if (o == Py_None) return true;
+    const Tensor* f = tensor(o, 1);
+    if (!f || f->numel() == 0 || 2 * f->numel() > dim || (f->scalar_type() != at::kDouble && f->scalar_type() != at::kFloat)) return false;
+    freq = *f;
+    return true;
+}
+
+// na_rotary(query, key, frequencies, positions | None, interleaved, magnitude)
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    if (n != 6 || at::impl::torch_function_mode_enabled()) return not_handled();
+    const Tensor *q = tensor(args[0], 4), *k = tensor(args[1], 4);
+    if (!q || !k || !spatial_equal(*q, *k, 1) || q->size(3) != k->size(3)) return not_handled();
+    OptTensor freq, positions;
+    bool interleaved;
+    std::optional<double> magnitude;
+    if (args[2] == Py_None || !turn(args[2], q->size(3), freq) || !boolean(args[4], interleaved) || !number(args[5], magnitude) || !magnitude)
+        return not_handled();
+    if (args[3] != Py_None) {
+        const Tensor *one = tensor(args[3], 1), *two = tensor(args[3], 2), *p = one ? one : two;
+        if (!p || !whole_numbers(*p) || p->size(-1) != q->size(1) || (two && p->size(0) != q->size(0))) return not_handled();
+        positions = *p;
+    }
+    std::tuple<Tensor, Tensor> r;
+    {
+        NoGil nogil;
+        r = call_rotary(*q, *k, *freq, positions, interleaved, *magnitude, false);
+    }
+    return pair_of(std::move(std::get<0>(r)), std::move(std::get<1>(r)));
+    END_HANDLE_TH_ERRORS
+}
+
+// caches, page table and lengths that fit each other and new tokens of `like`'s batch and head dim
+struct Cache { const Tensor *k, *v, *table, *lens; OptTensor seq_lens; };
+bool cache_args(PyObject* const* args, PyObject* seq_lens, const Tensor& like, Cache& c)
+{
+    c.k = tensor(args[0], 4);
+    c.v = tensor(args[1], 4);
+    c.table = tensor(args[2], 2);
+    c.lens = tensor(args[3], 1);
+    if (!c.k || !c.v || !c.table || !c.lens || c.k->sizes() != c.v->sizes() || c.k->size(3) != like.size(3) || c.k->size(1) < 1 ||
+        c.k->size(2) < 1 || !whole_numbers(*c.table) || !whole_numbers(*c.lens) || c.table->size(0) != like.size(0) || c.lens->size(0) != like.size(0))
+        return false;
+    if (seq_lens != Py_None) {
+        const Tensor* s = tensor(seq_lens, 1);
+        if (!s || !whole_numbers(*s) || s->size(0) != like.size(0)) return false;
+        c.seq_lens = *s;
+    }
+    return true;
+}
+
+// na_append(key, value, key_cache, value_cache, page_table, cache_lens, seq_lens | None, query | None, frequencies | None, interleaved,
+// magnitude)
+PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    if (n != 11 || at::impl::torch_function_mode_enabled()) return not_handled();
+    const Tensor *k = tensor(args[0], 4), *v = tensor(args[1], 4);
+    Cache c;
+    if (!k || !v || k->sizes() != v->sizes() || !cache_args(args + 2, args[6], *k, c) || k->size(2) != c.k->size(2)) return not_handled();
+    OptTensor query, freq;
+    if (args[7] != Py_None) {
+        const Tensor* q = tensor(args[7], 4);
+        if (!q || !spatial_equal(*q, *k, 1) || q->size(3) != k->size(3)) return not_handled();
+        query = *q;
+    }
+    bool interleaved;
+    std::optional<double> magnitude;
+    if (!turn(args[8], k->size(3), freq) || !boolean(args[9], interleaved) || !number(args[10], magnitude) || !magnitude) return not_handled();
+    Tensor out;
+    {
+        NoGil nogil;
+        out = call_append(*k, *v, *c.k, *c.v, *c.table, *c.lens, c.seq_lens, query, freq, interleaved, *magnitude);
+    }
+    if (!query) Py_RETURN_NONE;
+    return wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// na_paged(query, key_cache, value_cache, page_table, cache_lens, seq_lens | None, kernel_size | None, dilation, scale | None, return_lse)
+PyObject* py_paged(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    if (n != 10 || at::impl::torch_function_mode_enabled()) return not_handled();
+    const Tensor* q = tensor(args[0], 4);
+    Cache c;
+    if (!q || !cache_args(args + 1, args[5], *q, c) || q->size(2) % c.k->size(2) != 0 || q->size(2) < 1) return not_handled();
+    int64_t kernel[3] = {0, 0, 0}, dilation[3];
+    std::optional<double> scale;
+    bool want_lse;
+    if ((args[6] != Py_None && (!PyLong_CheckExact(args[6]) || !ints(args[6], 1, kernel))) || !PyLong_CheckExact(args[7]) ||
+        !ints(args[7], 1, dilation) || (args[6] == Py_None && dilation[0] != 1) || !number(args[8], scale) || !boolean(args[9], want_lse))
+        return not_handled();
+    if (!scale) scale = std::pow((double)q->size(-1), -0.5);
+    std::tuple<Tensor, Tensor> r;
+    {
+        NoGil nogil;
+        r = call_paged(*q, *c.k, *c.v, *c.table, *c.lens, c.seq_lens, kernel[0], dilation[0], *scale);
+    }
+    if (!want_lse) return wrap(std::move(std::get<0>(r)));
+    return pair_of(std::move(std::get<0>(r)), std::move(std::get<1>(r)));
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_set_flags(PyObject*, PyObject* o)
 {
     g_flags.store((int)PyLong_AsLong(o));
@@ -995,6 +1340,9 @@ PyMethodDef kMethods[] = {
     {"na_varlen", (PyCFunction)(void (*)(void))py_varlen, METH_FASTCALL, nullptr},
     {"na_qk", (PyCFunction)(void (*)(void))py_qk, METH_FASTCALL, nullptr},
     {"na_av", (PyCFunction)(void (*)(void))py_av, METH_FASTCALL, nullptr},
+    {"na_rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
+    {"na_append", (PyCFunction)(void (*)(void))py_append, METH_FASTCALL, nullptr},
+    {"na_paged", (PyCFunction)(void (*)(void))py_paged, METH_FASTCALL, nullptr},
     {"set_flags", py_set_flags, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -1013,6 +1361,9 @@ TORCH_LIBRARY_IMPL(natten_b200, CUDA, m)
     m.impl("na_qk_rpb_bwd", qk_rpb_bwd_cuda);
     m.impl("na_av", av_cuda);
     m.impl("na_av_bwd", av_bwd_cuda);
+    m.impl("na1d_rotary", rotary_cuda);
+    m.impl("na1d_append", append_cuda);
+    m.impl("na1d_paged", paged_cuda);
 }
 
 TORCH_LIBRARY_IMPL(natten_b200, Autograd, m)
@@ -1021,6 +1372,9 @@ TORCH_LIBRARY_IMPL(natten_b200, Autograd, m)
     m.impl("na_qk", qk_autograd);
     m.impl("na_qk_rpb", qk_rpb_autograd);
     m.impl("na_av", av_autograd);
+    m.impl("na1d_rotary", rotary_autograd);
+    m.impl("na1d_append", append_autograd);
+    m.impl("na1d_paged", paged_autograd);
 }
 
 PyMODINIT_FUNC PyInit__native(void) { return PyModule_Create(&kModule); }

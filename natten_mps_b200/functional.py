@@ -398,7 +398,133 @@ def na3d_varlen(query, key, value, spatial_sizes: torch.Tensor, kernel_size: Int
                       additional_keys, additional_values)
 
 
+# ---------------------------------------------------------------------------
+# around a decoder's cache: rotary positions, paged append, attention over the cache
+# ---------------------------------------------------------------------------
+def _check_index(t, shape, label: str) -> None:
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{label} must be a tensor of shape {list(shape)}, got "
+                         f"{list(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}.")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{label} must be int32 or int64, got {t.dtype}.")
+
+
+def _check_frequencies(frequencies, dim: int) -> None:
+    if frequencies.ndim != 1 or frequencies.dtype not in (torch.float32, torch.float64):
+        raise ValueError("frequencies must be a 1-D float64 (or float32) tensor, one entry per rotated channel pair.")
+    if not 1 <= frequencies.shape[0] <= dim // 2:
+        raise ValueError(f"frequencies must have between 1 and head_dim / 2 = {dim // 2} entries, got {frequencies.shape[0]}.")
+
+
+def _check_cache(name: str, like, key_cache, value_cache, page_table, cache_lens, seq_lens) -> None:
+    if key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError(f"{name} expects key_cache/value_cache with the same shape [pages, page_size, heads_kv, D].")
+    if key_cache.shape[1] < 1 or key_cache.shape[2] < 1:
+        raise ValueError("a cache's pages must hold at least one token of at least one head.")
+    if key_cache.shape[3] != like.shape[3]:
+        raise ValueError(f"Head dim must match between new tokens ({like.shape[3]}) and cache ({key_cache.shape[3]}).")
+    if page_table.ndim != 2 or page_table.shape[0] != like.shape[0]:
+        raise ValueError(f"page_table must be a [B={like.shape[0]}, pages per sequence] tensor, got {list(page_table.shape)}.")
+    _check_index(page_table, page_table.shape, "page_table")
+    _check_index(cache_lens, (like.shape[0],), "cache_lens")
+    if seq_lens is not None:
+        _check_index(seq_lens, (like.shape[0],), "seq_lens")
+
+
+def na1d_rotary(query, key, frequencies: torch.Tensor, positions: Optional[torch.Tensor] = None, *,
+                interleaved: bool = False, magnitude: float = 1.0):
+    """Rotary positions: ``query [B, L, Hq, D]`` and ``key [B, L, Hkv, D]`` with the first ``2 * len(frequencies)``
+    channels of every head turned by ``position * frequency`` radians and multiplied by ``magnitude``; the others are
+    copied.  Returns new (contiguous) tensors.
+
+    ``frequencies`` (float64, see ``rotary_frequencies``) and ``positions`` (int64 or int32, ``[L]`` or ``[B, L]``;
+    default ``0 ... L - 1``) are on the device and carry no gradient.  A pair is channels ``(i, i + n)`` of the ``n``
+    frequencies, or ``(2i, 2i + 1)`` when ``interleaved``.  Differentiable (any number of times) in query and key;
+    float32, float16, bfloat16 and float64, computed in float32 (float64) and rounded once."""
+    if not torch.compiler.is_compiling():
+        result = native.na_rotary(query, key, frequencies, positions, interleaved, magnitude)
+        if result is not NotImplemented:
+            return result
+    if query.ndim != 4 or key.ndim != 4 or query.shape[:2] != key.shape[:2] or query.shape[3] != key.shape[3]:
+        raise ValueError("na1d_rotary expects query [B, L, Hq, D] and key [B, L, Hkv, D] of the same B, L and D.")
+    _check_frequencies(frequencies, query.shape[3])
+    if positions is not None:
+        if positions.ndim not in (1, 2) or tuple(positions.shape) != tuple(query.shape[:2])[2 - positions.ndim:]:
+            raise ValueError(f"positions must be [L={query.shape[1]}] or [B={query.shape[0]}, L={query.shape[1]}], "
+                             f"got {list(positions.shape)}.")
+        _check_index(positions, positions.shape, "positions")
+    return torch.ops.natten_b200.na1d_rotary(query, key, frequencies, positions, bool(interleaved), float(magnitude), False)
+
+
+def na1d_append(key, value, key_cache, value_cache, page_table: torch.Tensor, cache_lens: torch.Tensor,
+                seq_lens: Optional[torch.Tensor] = None, *, query: Optional[torch.Tensor] = None,
+                frequencies: Optional[torch.Tensor] = None, interleaved: bool = False, magnitude: float = 1.0):
+    """Write the new tokens' ``key`` / ``value [B, L, Hkv, D]`` into a paged cache, in place; with ``frequencies`` the
+    keys (and ``query [B, L, Hq, D]``, when given) are rotated by their positions on the way (see ``na1d_rotary``).
+    Returns the rotated query (a copy without ``frequencies``; rows past ``seq_lens`` zero), or ``None`` without one.
+
+    ``key_cache`` / ``value_cache [pages, page_size, Hkv, D]`` may be strided (say, halves of one tensor) as long as the
+    channels are adjacent.  ``page_table [B, n]`` lists each sequence's pages, ``cache_lens [B]`` its tokens *with* the new
+    ones, ``seq_lens [B]`` how many of the ``L`` rows are new tokens (default: all): new token ``i`` goes to position
+    ``cache_lens - seq_lens + i``.  All three stay on the device (int32; int64 costs a conversion), so nothing is checked
+    against them on the host: a token whose position has no page (a negative or too large table entry, a position past the
+    table) is dropped, and the rest of the cache is left as it was.  Pages that are written to must belong to one sequence.
+    No backward pass: called with tensors that require grad (and grad enabled) it raises."""
+    if not torch.compiler.is_compiling():
+        result = native.na_append(key, value, key_cache, value_cache, page_table, cache_lens, seq_lens, query, frequencies,
+                                  interleaved, magnitude)
+        if result is not NotImplemented:
+            return result
+    if key.ndim != 4 or key.shape != value.shape:
+        raise ValueError("na1d_append expects key and value of the same shape [B, L, heads_kv, D].")
+    _check_cache("na1d_append", key, key_cache, value_cache, page_table, cache_lens, seq_lens)
+    if key.shape[2] != key_cache.shape[2]:
+        raise ValueError(f"key has {key.shape[2]} heads, the cache {key_cache.shape[2]}.")
+    if query is not None and (query.ndim != 4 or query.shape[:2] != key.shape[:2] or query.shape[3] != key.shape[3]):
+        raise ValueError("query must be [B, L, Hq, D] with key's B, L and D.")
+    if frequencies is not None:
+        _check_frequencies(frequencies, key.shape[3])
+    out = torch.ops.natten_b200.na1d_append(key, value, key_cache, value_cache, page_table, cache_lens, seq_lens, query,
+                                            frequencies, bool(interleaved), float(magnitude))
+    return out if query is not None else None
+
+
+def na1d_paged(query, key_cache, value_cache, page_table: torch.Tensor, cache_lens: torch.Tensor,
+               kernel_size: Optional[int] = None, dilation: int = 1, scale: Optional[float] = None,
+               return_lse: bool = False, *, seq_lens: Optional[torch.Tensor] = None):
+    """Causal 1-D neighbourhood attention of new tokens over a paged cache that holds them already (``na1d_append``).
+    ``query [B, L, Hq, D]``: from one token a sequence (a decoding step) to whole prompts, padded to ``L``; row ``i`` of
+    ``seq_lens[b]`` (default ``L``) stands at position ``p = cache_lens[b] - seq_lens[b] + i`` and sees the positions
+    ``p, p - dilation, ..., p - (kernel_size - 1) * dilation`` that exist, or all up to ``p`` with ``kernel_size=None``.
+    On a cache that holds a whole sequence this equals ``na1d(..., is_causal=True)`` on that sequence.
+
+    Returns ``[B, L, Hq, D]`` (with ``return_lse`` also the float32 log-sum-exp ``[B, L, Hq]``, as ``merge_attentions``
+    takes it).  Rows past ``seq_lens`` and rows that see nothing are zero with a log-sum-exp of -inf.  Caches, page table
+    and lengths as for ``na1d_append``; ``kernel_size`` may exceed the sequence.  A page that is not there (a negative or
+    too large entry: say, one given back because every window has passed it) is not attended to.  Float32, float16,
+    bfloat16; head dim up to 256; ``Hq % Hkv == 0``.  No backward pass: with tensors that require grad (and grad enabled)
+    it raises."""
+    if not torch.compiler.is_compiling():
+        result = native.na_paged(query, key_cache, value_cache, page_table, cache_lens, seq_lens, kernel_size, dilation, scale,
+                                 return_lse)
+        if result is not NotImplemented:
+            return result
+    if query.ndim != 4:
+        raise ValueError("na1d_paged expects query with shape [B, L, H, D].")
+    _check_cache("na1d_paged", query, key_cache, value_cache, page_table, cache_lens, seq_lens)
+    if query.shape[2] % key_cache.shape[2] != 0 or query.shape[2] < 1:
+        raise ValueError(f"heads_q ({query.shape[2]}) must be divisible by heads_kv ({key_cache.shape[2]}) for GQA.")
+    ks = 0 if kernel_size is None else normalize_kernel_size(kernel_size, 1)[0]
+    dil = normalize_tuple_param(dilation, 1, "dilation")[0]
+    if kernel_size is None and dil != 1:
+        raise ValueError("dilation needs a kernel_size.")
+    sc = query.shape[-1] ** -0.5 if scale is None else float(scale)
+    out, lse = torch.ops.natten_b200.na1d_paged(query, key_cache, value_cache, page_table, cache_lens, seq_lens, ks, dil, sc)
+    return (out, lse) if return_lse else out
+
+
 __all__ = [
+    "na1d_rotary", "na1d_append", "na1d_paged",
     "na1d_qk_rpb", "na2d_qk_rpb", "na3d_qk_rpb",
     "na1d", "na2d", "na3d", "na1d_qk", "na1d_av", "na2d_qk", "na2d_av", "na3d_qk", "na3d_av",
     "na1d_varlen", "na2d_varlen", "na3d_varlen",

@@ -15,6 +15,7 @@ import torch
 
 from .. import functional as F
 from .._torch_ops import native
+from ..rotary import rotary_frequencies
 from ..utils.params import normalize_tuple_param
 
 _FUSED = {1: F.na1d, 2: F.na2d, 3: F.na3d}
@@ -33,6 +34,7 @@ def _plain_linear(m) -> bool:
 
 class _NeighborhoodAttention(torch.nn.Module):
     rank = 0
+    _rotary = None               # rotary positions (1-D only): (frequencies by device, magnitude, interleaved)
 
     def __init__(self, embed_dim: int, num_heads: int, kernel_size: Union[int, Tuple[int, ...]],
                  stride: Union[int, Tuple[int, ...]] = 1, dilation: Union[int, Tuple[int, ...]] = 1,
@@ -98,11 +100,14 @@ class _NeighborhoodAttention(torch.nn.Module):
         if x.shape[-1] != self.embed_dim:
             raise ValueError(
                 f"Input channel dim ({x.shape[-1]}) must equal embed_dim ({self.embed_dim}).")
-        if sizes is None and self.attn_drop_p <= 0.0:
+        if sizes is None and self.attn_drop_p <= 0.0 and self._rotary is None:
             out = self._in_one_call(x)
             if out is not NotImplemented:
                 return out
         q, k, v = self._project(x)
+        if self._rotary is not None:
+            q, k = F.na1d_rotary(q, k, self._rotary.on(q.device), interleaved=self._rotary.interleaved,
+                                 magnitude=self._rotary.magnitude)
         if sizes is not None:
             out = _VARLEN[r](q, k, v, sizes, kernel_size=self.kernel_size, dilation=self.dilation,
                              scale=self.scale)
@@ -126,12 +131,56 @@ class _NeighborhoodAttention(torch.nn.Module):
         return self.proj_drop(self.proj(out))
 
 
+class _Rotary:
+    """Frequencies of a module's rotary positions.  Not a buffer: ``module.to(torch.bfloat16)`` would round them."""
+
+    def __init__(self, rotary_dim, base, interleaved, scaling):
+        self.values, self.magnitude = rotary_frequencies(rotary_dim, base, **(scaling or {}))
+        self.interleaved = bool(interleaved)
+        self._placed = {}
+
+    def on(self, device) -> torch.Tensor:
+        if device not in self._placed:
+            self._placed[device] = self.values.to(device)
+        return self._placed[device]
+
+
 class NeighborhoodAttention1D(_NeighborhoodAttention):
-    """1-D module; ``forward(x [B, L, C], seq_lens=None)``."""
+    """1-D module; ``forward(x [B, L, C], seq_lens=None)``.
+
+    ``rotary_dim > 0`` turns the first ``rotary_dim`` channels of every query and key head by their positions
+    (``rotary_base``, ``rotary_interleaved``; ``rotary_scaling``: keyword arguments of ``rotary_frequencies``).
+
+    ``forward(x, cache=layer)`` serves a decoder: ``x [B, L, C]`` are new tokens behind those that ``layer`` (a
+    ``PagedCache.layer``, extended for them) holds; their keys and values are appended, and they attend to the cache
+    through the module's causal window.  It needs ``is_causal``, unit stride and no gradients; attention dropout does not
+    apply."""
     rank = 1
 
-    def forward(self, x, seq_lens=None):  # noqa: D102
-        return super().forward(x, seq_lens)
+    def __init__(self, *args, rotary_dim: int = 0, rotary_base: float = 10000.0, rotary_interleaved: bool = False,
+                 rotary_scaling: Optional[dict] = None, **kwargs):
+        super().__init__(*args, **kwargs)
+        if rotary_dim:
+            if rotary_dim > self.head_dim:
+                raise ValueError(f"rotary_dim ({rotary_dim}) must not exceed head_dim ({self.head_dim}).")
+            self._rotary = _Rotary(rotary_dim, rotary_base, rotary_interleaved, rotary_scaling)
+
+    def forward(self, x, seq_lens=None, cache=None):  # noqa: D102
+        if cache is None:
+            return super().forward(x, seq_lens)
+        if seq_lens is not None:
+            raise ValueError("the cache knows the new tokens' seq_lens; give one of the two.")
+        if not self.is_causal[0] or self.stride[0] != 1:
+            raise ValueError("a cache needs is_causal=True and stride 1.")
+        if x.ndim != 3 or x.shape[-1] != self.embed_dim:
+            raise ValueError(f"NeighborhoodAttention1D expects input shape [B, L, C={self.embed_dim}].")
+        q, k, v = self._project(x)
+        turn = {} if self._rotary is None else {"frequencies": self._rotary.on(x.device), "interleaved": self._rotary.interleaved,
+                                                "magnitude": self._rotary.magnitude, "query": q}
+        turned = F.na1d_append(k, v, *cache, **turn)
+        out = F.na1d_paged(q if turned is None else turned, cache.key_cache, cache.value_cache, cache.page_table, cache.cache_lens,
+                           self.kernel_size[0], self.dilation[0], self.scale, seq_lens=cache.seq_lens)
+        return self.proj_drop(self.proj(out.reshape(*out.shape[:-2], self.embed_dim)))
 
 
 class NeighborhoodAttention2D(_NeighborhoodAttention):
