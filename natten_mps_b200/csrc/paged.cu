@@ -113,7 +113,10 @@ bool divide(Args& A, const Shape& shape)
     return true;
 }
 
-struct Chosen { Args A; bool aligned; };
+enum class Family { kGeneral, kWarp };
+struct Chosen { Args A; Family family; bool aligned; size_t workspace; };
+
+size_t workspace_of(const Args& A) { return (shared_bytes(A.ctas) + 2 * (size_t)A.ctas * slot_bytes(A.M, A.D) + 255) & ~(size_t)255; }
 
 int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void* kc, const void* vc)
 {
@@ -140,12 +143,24 @@ int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void*
     A.by_page = FastDiv((uint32_t)p->page_size);
     A.scale_log2 = (float)(p->scale * 1.4426950408889634);
     if (A.B == 0 || A.L == 0) return NATTEN_OK;
+    // The workspace serves every family that the call may take with other pointers and strides.
+    const bool simt = (p->flags & NATTEN_FLAG_FORCE_SIMT) != 0;
     Shape shape;
-    if (!general_shape(p->dtype, A, c.aligned, shape)) return NATTEN_E_UNSUPPORTED;
-    return divide(A, shape) ? NATTEN_OK : NATTEN_E_UNSUPPORTED;
+    Args general = A;
+    if (!general_shape(p->dtype, general, c.aligned, shape) || !divide(general, shape)) return NATTEN_E_UNSUPPORTED;
+    c.family = Family::kGeneral;
+    c.workspace = workspace_of(general);
+    if (!simt && warp_shape(p->dtype, A, p->dim % 8 == 0, shape)) {
+        if (!divide(A, shape)) return NATTEN_E_UNSUPPORTED;
+        c.workspace = std::max(c.workspace, workspace_of(A));
+        if (c.aligned) c.family = Family::kWarp;
+    }
+    if (c.family == Family::kGeneral) {
+        if (p->flags & NATTEN_FLAG_FORCE_TC) return NATTEN_E_UNSUPPORTED;
+        A = general;
+    }
+    return NATTEN_OK;
 }
-
-size_t workspace_of(const Args& A) { return (shared_bytes(A.ctas) + 2 * (size_t)A.ctas * slot_bytes(A.M, A.D) + 255) & ~(size_t)255; }
 
 } // namespace
 } // namespace paged
@@ -160,7 +175,7 @@ size_t natten_paged_workspace_bytes(const natten_paged_params_t* p)
 {
     Chosen c;
     if (choose(p, c, nullptr, nullptr, nullptr) != NATTEN_OK || c.A.B == 0 || c.A.L == 0) return 0;
-    return workspace_of(c.A);
+    return c.workspace;
 }
 
 int natten_paged_fwd(const natten_paged_params_t* p, const void* q, const void* k_cache, const void* v_cache, void* out, void* lse,
@@ -172,12 +187,12 @@ int natten_paged_fwd(const natten_paged_params_t* p, const void* q, const void* 
     Args& A = c.A;
     if (A.B == 0 || A.L == 0) return NATTEN_OK;
     if (!q || !out || !A.cache_lens || (A.table_width > 0 && !A.table) || (A.pages > 0 && (!k_cache || !v_cache))) return NATTEN_E_INVALID;
-    if (workspace_bytes < workspace_of(A) || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return NATTEN_E_WORKSPACE;
+    if (workspace_bytes < c.workspace || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return NATTEN_E_WORKSPACE;
     A.out = out;
     A.lse = static_cast<float*>(lse);
     A.ws = static_cast<unsigned char*>(workspace);
     const cudaStream_t s = (cudaStream_t)stream;
-    const int err = general_run(p->dtype, A, c.aligned, s);
+    const int err = c.family == Family::kWarp ? warp_run(p->dtype, A, s) : general_run(p->dtype, A, c.aligned, s);
     return err ? err : join(p->dtype, A, s);
 }
 
