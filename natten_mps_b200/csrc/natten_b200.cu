@@ -80,6 +80,9 @@ void set_vec_ok(Geo& g, int dtype, bool use_q, bool use_k, bool use_v, std::init
 int from_cuda(cudaError_t e) { return e == cudaSuccess ? NATTEN_OK : (int)e; }
 
 } // namespace
+
+void note_path(int path) { t_last_path = path; }
+
 } // namespace natten
 
 using namespace natten;

@@ -113,7 +113,7 @@ bool divide(Args& A, const Shape& shape)
     return true;
 }
 
-enum class Family { kGeneral, kWarp };
+enum class Family { kGeneral, kWarp, kTc };
 struct Chosen { Args A; Family family; bool aligned; size_t workspace; };
 
 size_t workspace_of(const Args& A) { return (shared_bytes(A.ctas) + 2 * (size_t)A.ctas * slot_bytes(A.M, A.D) + 255) & ~(size_t)255; }
@@ -150,15 +150,14 @@ int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void*
     if (!general_shape(p->dtype, general, c.aligned, shape) || !divide(general, shape)) return NATTEN_E_UNSUPPORTED;
     c.family = Family::kGeneral;
     c.workspace = workspace_of(general);
-    if (!simt && warp_shape(p->dtype, A, p->dim % 8 == 0, shape)) {
+    const bool tc = !simt && tc_shape(p->dtype, A, p->dim % 8 == 0, shape);
+    if (tc || (!simt && warp_shape(p->dtype, A, p->dim % 8 == 0, shape))) {
         if (!divide(A, shape)) return NATTEN_E_UNSUPPORTED;
         c.workspace = std::max(c.workspace, workspace_of(A));
-        if (c.aligned) c.family = Family::kWarp;
+        if (c.aligned) c.family = tc ? Family::kTc : Family::kWarp;
     }
-    if (c.family == Family::kGeneral) {
-        if (p->flags & NATTEN_FLAG_FORCE_TC) return NATTEN_E_UNSUPPORTED;
-        A = general;
-    }
+    if ((p->flags & NATTEN_FLAG_FORCE_TC) && c.family != Family::kTc) return NATTEN_E_UNSUPPORTED;
+    if (c.family == Family::kGeneral) A = general;
     return NATTEN_OK;
 }
 
@@ -192,7 +191,9 @@ int natten_paged_fwd(const natten_paged_params_t* p, const void* q, const void* 
     A.lse = static_cast<float*>(lse);
     A.ws = static_cast<unsigned char*>(workspace);
     const cudaStream_t s = (cudaStream_t)stream;
-    const int err = c.family == Family::kWarp ? warp_run(p->dtype, A, s) : general_run(p->dtype, A, c.aligned, s);
+    note_path(c.family == Family::kTc ? NATTEN_PATH_TCGEN05 : c.family == Family::kWarp ? NATTEN_PATH_WARP : NATTEN_PATH_SIMT);
+    const int err = c.family == Family::kTc ? tc_run(p->dtype, A, s) : c.family == Family::kWarp ? warp_run(p->dtype, A, s)
+                                                                                               : general_run(p->dtype, A, c.aligned, s);
     return err ? err : join(p->dtype, A, s);
 }
 

@@ -215,6 +215,14 @@ bool general_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int general_run(int dtype, const Args& A, bool aligned, cudaStream_t s);
 bool warp_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int warp_run(int dtype, const Args& A, cudaStream_t s);
+bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape);
+int tc_run(int dtype, const Args& A, cudaStream_t s);
+
+} // namespace paged
+
+void note_path(int path);        // what natten_last_path reports
+
+namespace paged {
 
 } // namespace paged
 } // namespace natten

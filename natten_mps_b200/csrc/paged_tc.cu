@@ -1,0 +1,701 @@
+// Attention over a paged cache for many rows a unit (chunks of a prompt, whole prompts), 16-bit types, head dims 64 and 128, on
+// tcgen05 tensor cores: one persistent CTA per SM, 128-key tiles.
+//
+//   S = Q K^T                     tcgen05.mma, 128 x 128, Q and K in shared memory, S in TMEM
+//   P = 2^(S scale log2(e) - m)   one thread a row, 32 columns at a time, written back as 16 bits over the scores they came from
+//   O += P V                      tcgen05.mma with A = P from TMEM, V read MN-major, O in TMEM
+//
+// Two row halves of 128 rows keep the tensor cores and the exponentials busy at the same time: while the threads of one half turn
+// its S into P, the products of the other run.  With more than 128 rows in a class the halves are rows 0 - 127 and 128 - 255 of
+// the unit and share every tile of keys; with fewer they take the same rows and every other tile of keys (kSplit), each with its
+// own maximum and sum, and are joined at the end.
+//
+// A row's maximum m is fixed at the first columns that it sees and moves only if a later score exceeds it by 2^60 (float16: 2^14),
+// which the row sum of a piece tells; O, the sum and the tile's probabilities so far are then rescaled by the thread itself.  So
+// there is no running maximum, and no thread has to touch O in between.
+//
+// Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products.  The rows of a tile lie anywhere
+// in the cache, so the loading threads look them up in the page table, a tile ahead, and copy them 16 bytes at a time
+// (asynchronously, two tiles in flight) into the swizzled layout that the tensor cores read; a row that is not there is zero.
+//
+// TMEM columns: S (P over its first half) of the halves at 0 and 128, O at 256 and 384.
+#include "../../include/natten_b200.h"
+
+#include "device_cache.cuh"
+#include "paged.cuh"
+#include "tc_common.cuh"
+#include "tc_kernels.cuh"
+#include "tc_plan.cuh"
+
+#include <math_constants.h>
+
+#include <type_traits>
+
+namespace natten {
+namespace paged {
+
+using namespace tc;
+using tcplan::add2;
+using tcplan::cvt_pack;
+using tcplan::fast_exp2;
+using tcplan::fma2;
+using tcplan::hi_of;
+using tcplan::lo_of;
+using tcplan::low_bits;
+using tcplan::pack2;
+using tcplan::transpose4;
+
+namespace {
+
+constexpr int kThreads = 512, kKeys = 128, kHalfRows = 128, kWordSlots = 16;
+constexpr int kSoftmaxRegs = 176, kHelperRegs = 80;              // 2 x 128 x (176 + 80) = the 65536 of the launch
+constexpr uint32_t kColO = 256;
+
+struct Status { int* status; int* status_host; long long wait_budget; int inject; };
+
+template <int DH, bool SPLIT> struct Cfg {
+    static constexpr int kBlocks = DH / 64;                      // 64-channel blocks: rows of 128 bytes, 128-byte swizzle
+    static constexpr int kRows = SPLIT ? kHalfRows : 2 * kHalfRows;
+    static constexpr int kQBlock = kRows * 128, kBlock = kKeys * 128;
+    static constexpr int kQ = kQBlock * kBlocks, kTile = kBlock * kBlocks;
+    static constexpr int kStages = DH == 128 ? (SPLIT ? 5 : 4) : 8;
+    static constexpr int kOffKV = kQ;
+    static constexpr int kOffRows = kOffKV + kStages * kTile;    // long long [3][2][kKeys]: places of a tile's keys and values
+    static constexpr int kOffWords = kOffRows + 3 * 2 * kKeys * 8;   // uint4 [kWordSlots]: which keys of a tile are there
+    static constexpr int kOffSums = kOffWords + kWordSlots * 16; // float2 [kHalfRows]: the second half's sums (kSplit)
+    static constexpr int kOffBars = kOffSums + kHalfRows * 8;
+    static constexpr int kBars = 2 * kStages + kWordSlots + 2 + 2 + 2 + 2 + 2 + 2;
+    static constexpr int kOffFlags = kOffBars + 8 * kBars;       // abort flag, TMEM address
+    static constexpr int kOffScratch = (kOffFlags + 8 + 15) & ~15;
+    static constexpr int kSmem = kOffScratch + 36 * 8;
+    static_assert(kSmem <= kMaxDynamicSmem, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
+{
+    const int n = there ? 16 : 0;            // 0: nothing is read, the chunk is zero
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// barrier 1 of the 128 loading threads; true if every one of them brought true
+__device__ __forceinline__ bool loaders_agree(bool ok)
+{
+    int all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((int)ok) : "memory");
+    return all != 0;
+}
+
+template <int DH, bool BF16, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Args A, const __grid_constant__ Status P)
+{
+    using C = Cfg<DH, SPLIT>;
+    constexpr int ST = C::kStages;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sbase = smem_u32(smem);
+    const int prior_abort = *reinterpret_cast<volatile int*>(P.status);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffFlags);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffFlags + 4);
+    uint32_t bar = sbase + C::kOffBars;
+    const uint32_t bar_full = bar;                               // [ST] a tile of keys or values has landed
+    const uint32_t bar_empty = bar_full + 8 * ST;                // [ST] ... its products are done
+    const uint32_t bar_words = bar_empty + 8 * ST;               // [kWordSlots] which keys of the tile are there
+    const uint32_t bar_q = bar_words + 8 * kWordSlots;           // Q of the unit has landed
+    const uint32_t bar_qfree = bar_q + 8;                        // the unit's last S is done
+    const uint32_t bar_s = bar_qfree + 8;                        // [2] S of the half's tile is in TMEM, and every earlier product is done
+    const uint32_t bar_p = bar_s + 16;                           // [2] every thread of the half stored its P
+    const uint32_t bar_o = bar_p + 16;                           // [2] the half's last P V of the unit is done
+    const uint32_t bar_ofree = bar_o + 16;                       // [2] O has been read
+    const uint32_t bar_sums = bar_ofree + 16;                    // [2] kSplit: the second half's sums are in shared memory; have been read
+
+    if (warp == 12) {
+        if (lane == 0) {
+            // swizzled tiles need a 1024-byte aligned base; once any CTA has given up, the rest bail out
+            *abort_flag = ((sbase & 1023u) || prior_abort) ? 1 : 0;
+            for (int i = 0; i < ST; ++i) {
+                mbar_init(bar_full + 8 * i, 128);
+                mbar_init(bar_empty + 8 * i, 1);
+            }
+            for (int i = 0; i < kWordSlots; ++i) mbar_init(bar_words + 8 * i, 4);
+            mbar_init(bar_q, 128);
+            mbar_init(bar_qfree, 1);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(bar_s + 8 * i, 1);
+                mbar_init(bar_p + 8 * i, 128);
+                mbar_init(bar_o + 8 * i, 1);
+                mbar_init(bar_ofree + 8 * i, 128);
+                mbar_init(bar_sums + 8 * i, 128);
+            }
+            mbar_init_fence();
+            fence_async_smem();
+        }
+        __syncwarp();
+        tmem_alloc(smem_u32(tmem_slot), 512);
+    }
+    Piece piece;
+    piece.begin<kThreads>(A, blockIdx.x, smem + C::kOffScratch);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    Shared told{-1, -1, 0, 0};
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+        if (warp == 12) {
+            // =====================================================================
+            // MMA issue: the whole warp walks the units, the instructions execute on one elected lane.
+            // =====================================================================
+            bool ok = !gave_up(abort_flag);
+            constexpr uint32_t idesc_qk = instr_desc(BF16 ? 1 : 0, kKeys, 0, 0), idesc_pv = instr_desc(BF16 ? 1 : 0, DH, 0, 1);
+            const uint32_t leader = elect_one();
+            unsigned fills = 0, units[2] = {0, 0}, tiles[2] = {0, 0};           // tiles of keys and values taken; units, tiles of each half
+            unsigned queries = 0;
+            for (; ok && piece.more(); piece.advance(A)) {
+                const Piece::Portion p = piece.portion(A);
+                if (!p.work) continue;
+                const int n = p.x1 - p.x0;
+                const bool two = SPLIT ? n > 1 : piece.tile.rows > kHalfRows;
+                auto wait_full = [&]() { ok = ok && mbar_wait(bar_full + 8 * (fills % ST), (fills / ST) & 1, abort_flag, P.wait_budget); };
+                auto scores = [&](int half) {
+                    const uint64_t dq = smem_desc(sbase + (SPLIT ? 0 : half * kHalfRows * 128), 16, 1024),
+                                   dk = smem_desc(sbase + C::kOffKV + (fills % ST) * C::kTile, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < DH / 16; ++k)            // 32 bytes per step inside a 64-channel block
+                        mma_ss_e(tmem + 128 * half, dq + (((k / 4) * C::kQBlock + (k % 4) * 32) >> 4),
+                                 dk + (((k / 4) * C::kBlock + (k % 4) * 32) >> 4), idesc_qk, k > 0, leader);
+                    mma_commit_e(bar_s + 8 * half, leader);
+                };
+                auto weighted = [&](int half, bool first) {
+                    const uint64_t dv = smem_desc(sbase + C::kOffKV + (fills % ST) * C::kTile, C::kBlock, 1024);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)         // 16 keys per step: 16 rows of V, 8 columns of P
+                        mma_ts_e(tmem + kColO + 128 * half, tmem + 128 * half + 8 * k, dv + 128 * k, idesc_pv, (!first || k > 0) ? 1u : 0u, leader);
+                };
+                auto release = [&]() {
+                    mma_commit_e(bar_empty + 8 * (fills % ST), leader);
+                    ++fills;
+                };
+                auto wait_p = [&](int half, bool first) {
+                    if (first && units[half] > 0) ok = ok && mbar_wait(bar_ofree + 8 * half, (units[half] - 1) & 1, abort_flag, P.wait_budget);
+                    ok = ok && mbar_wait(bar_p + 8 * half, tiles[half] & 1, abort_flag, P.wait_budget);
+                    ++tiles[half];
+                };
+                ok = ok && mbar_wait(bar_q, queries & 1, abort_flag, P.wait_budget);
+                ++queries;
+                wait_full();
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                if constexpr (SPLIT) {
+                    // tile j belongs to half j & 1; order of the loads: K0, K1, V0, K2, V1, ...
+                    scores(0);
+                    if (n == 1) mma_commit_e(bar_qfree, leader);
+                    release();
+                    for (int j = 0; j < n; ++j) {
+                        if (j + 1 < n) {
+                            wait_full();
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores((j + 1) & 1);                 // after P V of tile j - 1 in issue order: over its P
+                            if (j + 2 == n) mma_commit_e(bar_qfree, leader);
+                            release();
+                        }
+                        wait_full();
+                        wait_p(j & 1, j < 2);
+                        if (!ok) break;
+                        tc_fence_after();
+                        weighted(j & 1, j < 2);
+                        release();
+                        if (j + 2 >= n) mma_commit_e(bar_o + 8 * (j & 1), leader);
+                    }
+                } else {
+                    // both halves use every tile; order of the loads: K0, V0, K1, V1, ...
+                    scores(0);
+                    if (two) scores(1);
+                    if (n == 1) mma_commit_e(bar_qfree, leader);
+                    release();
+                    for (int j = 0; j < n; ++j) {
+                        const unsigned v = fills;                // V of the tile; K of the next one follows it
+                        auto next_scores = [&](int half) {
+                            if (j + 1 == n) return;
+                            fills = v + 1;
+                            if (half == 0) wait_full();
+                            if (ok) {
+                                tc_fence_after();
+                                scores(half);
+                            }
+                            fills = v;
+                        };
+                        wait_full();
+                        wait_p(0, j == 0);
+                        if (!ok) break;
+                        tc_fence_after();
+                        weighted(0, j == 0);
+                        if (j + 1 == n) mma_commit_e(bar_o, leader);
+                        next_scores(0);
+                        if (two) {
+                            wait_p(1, j == 0);
+                            if (!ok) break;
+                            tc_fence_after();
+                            weighted(1, j == 0);
+                            if (j + 1 == n) mma_commit_e(bar_o + 8, leader);
+                        }
+                        release();                               // V
+                        if (j + 1 < n) {
+                            fills = v;
+                            if (two) next_scores(1);
+                            fills = v + 1;
+                            if (j + 2 == n) mma_commit_e(bar_qfree, leader);
+                            release();                           // K of the next tile
+                        }
+                    }
+                }
+                ++units[0];
+                if (two) ++units[1];
+                if (!__all_sync(0xffffffffu, ok)) ok = false;    // the lanes agree once a unit
+            }
+        } else if (warp < 12) {
+            // =====================================================================
+            // Loads
+            // =====================================================================
+            const int lt = tid - 256;
+            const uint16_t *q = static_cast<const uint16_t*>(A.q), *kc = static_cast<const uint16_t*>(A.kc), *vc = static_cast<const uint16_t*>(A.vc);
+            long long* places = reinterpret_cast<long long*>(smem + C::kOffRows);      // [3][K: kKeys, V: kKeys]
+            constexpr int kChunks = DH / 8, kAtOnce = 128 / kChunks;   // 16-byte chunks of a row; rows at a time
+            const int c = lt % kChunks, r0 = lt / kChunks;
+            const uint32_t c_off = (c >> 3) * C::kBlock, cq_off = (c >> 3) * C::kQBlock;
+            bool ok = loaders_agree(!*abort_flag);
+            unsigned fills = 0, seq = 0, queries = 0;
+            uint32_t waiting[2] = {0u, 0u};                      // barriers of the copies in flight, oldest first
+            int in_flight = 0;
+            auto arrive = [&](uint32_t b) {
+                fence_async_smem();                              // what this thread copied is read by the tensor cores
+                if (b) mbar_arrive(b);
+            };
+            auto flush = [&]() {
+                copies_wait<0>();
+                if (in_flight > 0) arrive(waiting[0]);
+                if (in_flight > 1) arrive(waiting[1]);
+                in_flight = 0;
+            };
+            auto issued = [&](uint32_t b) {                      // copies are under way; their barrier is told two fills later
+                copies_commit();
+                if (in_flight == 2) {
+                    copies_wait<2>();
+                    arrive(waiting[0]);
+                    waiting[0] = waiting[1];
+                    in_flight = 1;
+                }
+                waiting[in_flight++] = b;
+            };
+            auto wait_empty = [&](uint32_t b, uint32_t parity) { // nothing may be held back while this thread waits for the consumers
+                if (ok && !mbar_try_wait(b, parity)) {
+                    flush();
+                    ok = mbar_wait(b, parity, abort_flag, P.wait_budget);
+                }
+            };
+            auto fill = [&](const uint16_t* src, const long long* place) {
+                const unsigned s = fills % ST;
+                if (fills >= (unsigned)ST) wait_empty(bar_empty + 8 * s, (fills / ST - 1) & 1);
+                if (ok) {
+                    const uint32_t dst = sbase + C::kOffKV + s * C::kTile + c_off;
+#pragma unroll 4
+                    for (int r = r0; r < kKeys; r += kAtOnce) {
+                        const long long o = place[r];
+                        copy16(dst + r * 128 + (((c ^ r) & 7) << 4), o >= 0 ? src + o + c * 8 : q, o >= 0);
+                    }
+                    issued(bar_full + 8 * s);
+                }
+                ++fills;
+            };
+            for (; ok && piece.more(); piece.advance(A)) {
+                const Piece::Portion p = piece.portion(A);
+                if (!p.work) continue;
+                const Tile& x = piece.tile;
+                const int n = p.x1 - p.x0;
+                int page = 0, slot = 0;
+                bool there = locate(A, x, x.lo + p.x0 * kKeys + lt, page, slot);
+                // Places of tile j (the lookup for the next one is under way while this one is copied).  Three buffers: with kSplit
+                // a thread may still copy the values of tile j - 2 when another writes the places of tile j.
+                auto place_tile = [&](int j) {
+                    long long* at = places + (j % 3) * 2 * kKeys;
+                    at[lt] = there ? page * A.ks[0] + slot * A.ks[1] + p.h * A.ks[2] : -1;
+                    at[kKeys + lt] = there ? page * A.vs[0] + slot * A.vs[1] + p.h * A.vs[2] : -1;
+                    const unsigned seen = __ballot_sync(0xffffffffu, there), w = seq % kWordSlots;
+                    if (lane == 0) {
+                        reinterpret_cast<unsigned*>(smem + C::kOffWords)[4 * w + (warp & 3)] = seen;
+                        mbar_arrive(bar_words + 8 * w);
+                    }
+                    ++seq;
+                    there = j + 1 < n && locate(A, x, x.lo + (p.x0 + j + 1) * kKeys + lt, page, slot);
+                    ok = loaders_agree(ok);
+                    return at;
+                };
+                auto load_queries = [&]() {
+                    if (queries > 0) wait_empty(bar_qfree, (queries - 1) & 1);
+                    if (ok) {
+#pragma unroll 2
+                        for (int r = r0; r < C::kRows; r += kAtOnce) {
+                            const bool here = r < x.rows;
+                            copy16(sbase + cq_off + r * 128 + (((c ^ r) & 7) << 4), here ? q + query_offset(A, x, p.h, r) + c * 8 : q, here);
+                        }
+                        issued(P.inject == 1 && queries == 0 && lt == 0 ? 0u : bar_q);      // test hook: a barrier that never fills
+                    }
+                    ++queries;
+                };
+                const long long* at = place_tile(0);
+                if (!ok) break;
+                fill(kc, at);
+                load_queries();
+                if constexpr (SPLIT) {
+                    for (int j = 0; j < n; ++j) {
+                        const long long* next = nullptr;
+                        if (j + 1 < n) {
+                            next = place_tile(j + 1);
+                            if (!ok) break;
+                            fill(kc, next);
+                        }
+                        fill(vc, at + kKeys);
+                        at = next;
+                    }
+                } else {
+                    for (int j = 0; j < n; ++j) {
+                        fill(vc, at + kKeys);
+                        if (j + 1 < n) {
+                            at = place_tile(j + 1);
+                            if (!ok) break;
+                            fill(kc, at);
+                        }
+                    }
+                }
+                ok = loaders_agree(ok);                          // the places have been read by everyone
+            }
+            flush();
+        }
+    } else {
+        // =====================================================================
+        // Softmax and output: a thread a row
+        // =====================================================================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        constexpr float kGrow = BF16 ? 60.f : 14.f;              // headroom of the stored probabilities, as an exponent
+        constexpr float kGrowSum = BF16 ? 1.152921504606847e18f : 16384.f;     // 2^kGrow: a piece's sum below it has none above it
+        const int half = warp >> 2, row = (SPLIT ? 0 : half * kHalfRows) + (warp & 3) * 32 + lane;
+        const uint32_t trow = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), scol = trow + 128 * half, ocol = trow + kColO + 128 * half;
+        float2* sums = reinterpret_cast<float2*>(smem + C::kOffSums);
+        bool ok = !gave_up(abort_flag);
+        unsigned mine = 0, seq = 0, units = 0, exchanges = 0;    // tiles of this half, tiles of the CTA, units of this half
+        const uint64_t sc2 = pack2(A.scale_log2, A.scale_log2);
+        for (; ok && piece.more(); piece.advance(A)) {
+            const Piece::Portion p = piece.portion(A);
+            const Tile& x = piece.tile;
+            const bool clear = x.n == 0 && p.first;
+            if (!p.work && !clear) continue;
+            const int n = p.work ? p.x1 - p.x0 : 0;
+            const bool direct = clear || p.whole;
+            const int where = 2 * (int)blockIdx.x + (p.x0 == 0 ? 1 : 0);
+            if (!direct) {
+                const int unit = piece.column * A.Hkv + p.h;
+                if (p.x0 == 0) told.tail = unit;
+                else {
+                    told.head = unit;
+                    told.head_done = p.x1 == x.n;
+                }
+            }
+            const bool active = SPLIT ? half == 0 || n > 1 : half == 0 || x.rows > kHalfRows;
+            if (!active) {
+                seq += n;
+                continue;
+            }
+            long long index = -1;
+            int tq = -1;
+            const bool in_tile = row < x.rows;
+            bool live = in_tile && row_of(A, x, p.h, row, index, tq);
+            if (!in_tile) index = -1;
+            const int t_least = __reduce_min_sync(0xffffffffu, live ? tq : 0x7fffffff), t_most = __reduce_max_sync(0xffffffffu, live ? tq : -1);
+            if (!live) tq = -1;
+            float m = -CUDART_INF_F, l = 0.f;
+            // rare: a score far above the maximum.  Move it; rescale O (its products so far are done, see bar_s), the sum and the
+            // probabilities of this tile's first `pieces` pieces.
+            auto rescale = [&](bool grow, float over, bool had_tiles, int pieces) {
+                const float f = grow ? fast_exp2(-over) : 1.f;
+                tmem_st_wait();
+                if (had_tiles) {
+#pragma unroll 1
+                    for (int part = 0; part < DH / 16; ++part) {
+                        uint32_t o[16];
+                        tmem_ld16(ocol + 16 * part, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(ocol + 16 * part, o);
+                    }
+                }
+#pragma unroll 1
+                for (int pc = 0; pc < pieces; ++pc) {
+                    uint32_t w[16];
+                    tmem_ld16(scol + 16 * pc, w);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float a, b;
+                        if (BF16) {
+                            a = __uint_as_float(w[i] << 16);
+                            b = __uint_as_float(w[i] & 0xffff0000u);
+                        } else {
+                            const __half2 h2 = *reinterpret_cast<const __half2*>(&w[i]);
+                            a = __low2float(h2);
+                            b = __high2float(h2);
+                        }
+                        w[i] = cvt_pack<BF16>(a * f, b * f);
+                    }
+                    tmem_st16(scol + 16 * pc, w);
+                }
+                l *= f;
+                if (grow) m += over;
+            };
+            bool had_tiles = false;
+            for (int j = 0; j < n; ++j, ++seq) {
+                if (SPLIT && (j & 1) != half) continue;
+                const int base = x.lo + (p.x0 + j) * kKeys;
+                const unsigned w = seq % kWordSlots;
+                ok = ok && mbar_wait(bar_words + 8 * w, (seq / kWordSlots) & 1, abort_flag, P.wait_budget);
+                const volatile uint32_t* there_words = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffWords) + 4 * w;
+                const uint32_t words[4] = {there_words[0], there_words[1], there_words[2], there_words[3]};
+                ok = ok && mbar_wait(bar_s + 8 * half, mine & 1, abort_flag, P.wait_budget);
+                ++mine;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int pc = 0; pc < 4; ++pc) {
+                    const int t0 = base + 32 * pc;
+                    uint32_t pk[16];
+                    if (t0 > t_most || (t0 + 31 < t_least && t_least - (t0 + 31) >= A.K)) {       // no row of the warp sees the piece
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) pk[i] = 0u;
+                        tmem_st16(scol + 16 * pc, pk);
+                        continue;
+                    }
+                    uint32_t s[32];
+                    tmem_ld32(scol + 32 * pc, s);
+                    tmem_ld_wait();
+                    // every row of the warp that counts sees all of the piece
+                    const bool open = words[pc] == 0xffffffffu && t0 + 31 <= t_least && t_most - t0 < A.K;
+                    uint32_t bits = 0xffffffffu;
+                    if (!open) bits = low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & words[pc];
+                    bool done = false;
+                    if (open && !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
+                        const uint64_t nb2 = pack2(-m, -m);
+                        uint64_t sum = 0ull;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t e = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, nb2);
+                            const float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e));
+                            sum = add2(sum, pack2(a, b));
+                            pk[i] = cvt_pack<BF16>(a, b);
+                        }
+                        const float rs = lo_of(sum) + hi_of(sum);
+                        if (!__any_sync(0xffffffffu, !(rs <= kGrowSum))) {
+                            l += rs;
+                            done = true;
+                        }
+                    }
+                    if (!done) {
+                        if (m == -CUDART_INF_F && bits != 0u) {  // first columns that the row sees
+                            float top = -CUDART_INF_F;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * A.scale_log2);
+                            m = top;
+                        }
+                        const float base_m = m == -CUDART_INF_F ? 0.f : m;
+                        float over = -CUDART_INF_F;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float e = (bits >> i) & 1u ? fmaf(__uint_as_float(s[i]), A.scale_log2, -base_m) : -CUDART_INF_F;
+                            s[i] = __float_as_uint(e);
+                            over = fmaxf(over, e);
+                        }
+                        const bool grow = over > kGrow;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            rescale(grow, over, had_tiles, pc);
+                            if (grow) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - over);
+                            }
+                        }
+                        float sum_a = 0.f, sum_b = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float a = fast_exp2(__uint_as_float(s[2 * i])), b = fast_exp2(__uint_as_float(s[2 * i + 1]));
+                            sum_a += a;
+                            sum_b += b;
+                            pk[i] = cvt_pack<BF16>(a, b);
+                        }
+                        l += sum_a + sum_b;
+                    }
+                    tmem_st16(scol + 16 * pc, pk);               // over columns of this thread's that have been read
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(bar_p + 8 * half);
+                had_tiles = true;
+            }
+            if (!ok) break;
+
+            // ---- output ----
+            float f_mine = 1.f, f_other = 0.f;
+            if (n > 0) {
+                if (SPLIT && half == 1) {
+                    if (exchanges > 0) ok = ok && warp_wait(bar_sums + 8, (exchanges - 1) & 1, abort_flag, P.wait_budget);
+                    if (!ok) break;
+                    sums[(warp & 3) * 32 + lane] = make_float2(m, l);
+                    mbar_arrive(bar_sums);
+                    ++exchanges;
+                    ++units;
+                    continue;                                    // the first half writes the rows
+                }
+                if (SPLIT && n > 1) {
+                    ok = warp_wait(bar_sums, exchanges & 1, abort_flag, P.wait_budget) && ok;
+                    ok = ok && warp_wait(bar_o + 8, exchanges & 1, abort_flag, P.wait_budget);
+                    if (!ok) break;
+                    const float2 other = sums[(warp & 3) * 32 + lane];
+                    mbar_arrive(bar_sums + 8);
+                    ++exchanges;
+                    const float top = fmaxf(m, other.x), base_m = top == -CUDART_INF_F ? 0.f : top;
+                    f_mine = fast_exp2(m - base_m);
+                    f_other = fast_exp2(other.x - base_m);
+                    l = l * f_mine + other.y * f_other;
+                    m = top;
+                }
+                ok = ok && warp_wait(bar_o + 8 * half, units & 1, abort_flag, P.wait_budget);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const bool some = live && l != 0.f;                  // (a NaN stays one)
+            const float inv = direct ? (some ? 1.f / l : 0.f) : 1.f;
+            const bool both = SPLIT && n > 1;
+            // Four lanes exchange 16-byte pieces, so that a store writes 64 bytes of each of eight rows.
+            long long rows4[4];
+            const long long my_row = direct ? index : in_tile ? row : -1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rows4[i] = __shfl_sync(0xffffffffu, my_row, (lane & ~3) | i);
+            const int piece4 = lane & 3;
+#pragma unroll 1
+            for (int part = 0; part < DH / 32; ++part) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld32(ocol + 32 * part, o);
+                    tmem_ld_wait();
+                    if (both) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t y[16];
+                            tmem_ld16(trow + kColO + 128 + 32 * part + 16 * h, y);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                o[16 * h + i] = __float_as_uint(__uint_as_float(o[16 * h + i]) * f_mine + __uint_as_float(y[i]) * f_other);
+                        }
+                    }
+                }
+                if (direct) {
+                    uint32_t y[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            y[i][k] = some ? cvt_pack<BF16>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv) : 0u;
+                    transpose4(y, piece4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (rows4[i] >= 0)
+                            reinterpret_cast<uint4*>(static_cast<uint16_t*>(A.out) + rows4[i] * DH)[4 * part + piece4] =
+                                make_uint4(y[i][0], y[i][1], y[i][2], y[i][3]);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t y[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) y[i][k] = o[16 * h + 4 * i + k];
+                        transpose4(y, piece4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (rows4[i] >= 0)
+                                reinterpret_cast<uint4*>(slot_out(A, where) + rows4[i] * DH)[8 * part + 4 * h + piece4] =
+                                    make_uint4(y[i][0], y[i][1], y[i][2], y[i][3]);
+                    }
+                }
+            }
+            if (in_tile) {
+                if (!direct) slot_sums(A, where)[row] = make_float2(live ? m : -CUDART_INF_F, live ? l : 0.f);
+                else if (A.lse) A.lse[index] = some ? (m + log2f(l)) * 0.6931471805599453f : -CUDART_INF_F;
+            }
+            if (n > 0) {
+                tc_fence_before();
+                mbar_arrive(bar_ofree + 8 * half);
+                if (both) mbar_arrive(bar_ofree + 8);
+                ++units;
+            }
+        }
+        if (tid == 0) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
+    }
+
+    if (*abort_flag) abort_grace_sleep();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+        if (lane == 0 && *abort_flag) tcplan::raise_status(P);
+    }
+}
+
+} // namespace
+
+bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape)
+{
+    if ((dtype != NATTEN_F16 && dtype != NATTEN_BF16) || !aligned || (A.D != 64 && A.D != 128)) return false;
+    const long long rows = ((long long)A.L + A.dil - 1) / A.dil * A.G;
+    if (rows <= 32) return false;
+    shape = {rows > kHalfRows ? 2 * kHalfRows : kHalfRows, kKeys, 1, 2, sm_count()};
+    return true;
+}
+
+int tc_run(int dtype, const Args& A, cudaStream_t s)
+{
+    Status st{};
+    st.wait_budget = tcplan::debug_wait_budget();
+    st.inject = tcplan::debug_inject();
+    cudaError_t err = tcplan::status_ptr(st.status);
+    if (err == cudaSuccess) err = tcplan::status_host_ptr(st.status_host);
+    if (err != cudaSuccess) return (int)err;
+    auto go = [&](auto dh, auto bf, auto split) {
+        constexpr int kDim = decltype(dh)::value;
+        using C = Cfg<kDim, decltype(split)::value>;
+        auto* kernel = tc_kernel<kDim, decltype(bf)::value, decltype(split)::value>;
+        err = ensure_dynamic_smem((const void*)kernel, C::kSmem);
+        if (err == cudaSuccess) kernel<<<A.ctas, kThreads, C::kSmem, s>>>(A, st);
+    };
+    auto by_rows = [&](auto dh, auto bf) {
+        if (A.M == kHalfRows) go(dh, bf, std::true_type{});
+        else go(dh, bf, std::false_type{});
+    };
+    auto by_dim = [&](auto bf) {
+        if (A.D == 64) by_rows(std::integral_constant<int, 64>{}, bf);
+        else by_rows(std::integral_constant<int, 128>{}, bf);
+    };
+    if (dtype == NATTEN_BF16) by_dim(std::true_type{});
+    else by_dim(std::false_type{});
+    if (err == cudaSuccess) err = cudaGetLastError();
+    tc_count_launch();
+    return (int)err;
+}
+
+} // namespace paged
+} // namespace natten

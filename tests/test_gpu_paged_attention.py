@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from natten_mps_b200 import functional as F
+from natten_mps_b200 import _cabi, functional as F
 from tests import _decoder_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -210,3 +210,47 @@ def test_equals_attention_on_the_whole_sequence():
         for rows in (L, 1, 40):
             got, lse = F.na1d_paged(q[:, L - rows:], *caches, table, lens, kernel, dilation, return_lse=True)
             assert (got - want[:, L - rows:]).abs().max() <= 1e-5 and (lse - want_lse[:, L - rows:]).abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("L,group", [(70, 4), (40, 2)], ids=["rows", "split_keys"])
+def test_wait_that_runs_out_is_reported_and_recoverable(L, group):
+    """The queries' barrier never fills (made on the host): the kernel gives up, says so, and the next call works again."""
+    q, k_cache, v_cache, table, lens, new = [t.cuda() for t in _problem(BF16, [300, 200], [L, L], L, 2 * group, 2, 64, 16, poison=False)]
+    call = lambda: F.na1d_paged(q, k_cache, v_cache, table, lens)  # noqa: E731
+    try:
+        want = call()
+        assert _cabi.last_path() == "tcgen05"
+        _cabi.lib().natten_debug_wait(400_000, 1)
+        call()
+        torch.cuda.synchronize()
+        assert _cabi.device_status() == -4
+        _cabi.lib().natten_debug_wait(0, 0)
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            call()
+        _cabi.clear_status()
+        got = call()
+        torch.cuda.synchronize()
+        assert _cabi.device_status() == 0 and torch.equal(got, want)
+    finally:
+        _cabi.lib().natten_debug_wait(0, 0)
+        _cabi.clear_status()
+
+
+def test_paths():
+    """Which kernels serve a call: rows a class, type, alignment, and the testing flags."""
+    def path(dtype, L, Hq, Hkv, D, kernel=None, dilation=1):
+        q, k_cache, v_cache, table, lens, new = [t.cuda() for t in _problem(dtype, [100], [L], L, Hq, Hkv, D, 16, poison=False)]
+        F.na1d_paged(q, k_cache, v_cache, table, lens, kernel, dilation)
+        return _cabi.last_path()
+
+    assert path(BF16, 1, 16, 4, 128) == "warp" and path(F16, 100, 8, 2, 128) == "tcgen05" and path(BF16, 50, 4, 2, 64) == "tcgen05"
+    assert path(BF16, 50, 4, 2, 96) == "warp" and path(F32, 1, 4, 2, 64) == "simt" and path(BF16, 1, 4, 2, 20) == "simt"
+    assert path(BF16, 64, 2, 2, 64, 5, 64) == "warp"                 # a row a class
+    try:
+        _cabi.set_force("simt")
+        assert path(BF16, 100, 8, 2, 128) == "simt"
+        _cabi.set_force("tc")
+        with pytest.raises(NotImplementedError):
+            path(BF16, 1, 16, 4, 128)
+    finally:
+        _cabi.set_force(None)
