@@ -16,7 +16,7 @@
 //
 // Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products.  The rows of a tile lie anywhere
 // in the cache, so the loading threads look them up in the page table, a tile ahead, and copy them 16 bytes at a time
-// (asynchronously, two tiles in flight) into the swizzled layout that the tensor cores read; a row that is not there is zero.
+// (asynchronously, as far ahead as the stages go) into the swizzled layout that the tensor cores read; a row that is not there is zero.
 //
 // TMEM columns: S (P over its first half) of the halves at 0 and 128, O at 256 and 384.
 #include "../../include/natten_b200.h"
@@ -76,8 +76,22 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there
     const int n = there ? 16 : 0;            // 0: nothing is read, the chunk is zero
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// The barrier gets this thread's arrival once all copies that it has issued so far have landed.  They are ordinary writes: who reads
+// them through the tensor cores puts a proxy fence behind its wait.
+__device__ __forceinline__ void arrive_when_landed(uint32_t b)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b) : "memory");
+}
+// The loads of this thread's TMEM rows have landed: nothing that uses them may move in front of this.
+__device__ __forceinline__ void landed(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
 // barrier 1 of the 128 loading threads; true if every one of them brought true
 __device__ __forceinline__ bool loaders_agree(bool ok)
 {
@@ -188,6 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 wait_full();
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                fence_async_smem();
                 tc_fence_after();
                 if constexpr (SPLIT) {
                     // tile j belongs to half j & 1; order of the loads: K0, K1, V0, K2, V1, ...
@@ -198,12 +213,14 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         if (j + 1 < n) {
                             wait_full();
                             if (!ok) break;
+                            fence_async_smem();
                             tc_fence_after();
                             scores((j + 1) & 1);                 // after P V of tile j - 1 in issue order: over its P
                             if (j + 2 == n) mma_commit_e(bar_qfree, leader);
                             release();
                         }
                         wait_full();
+                        fence_async_smem();
                         wait_p(j & 1, j < 2);
                         if (!ok) break;
                         tc_fence_after();
@@ -224,12 +241,14 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             fills = v + 1;
                             if (half == 0) wait_full();
                             if (ok) {
+                                if (half == 0) fence_async_smem();
                                 tc_fence_after();
                                 scores(half);
                             }
                             fills = v;
                         };
                         wait_full();
+                        fence_async_smem();
                         wait_p(0, j == 0);
                         if (!ok) break;
                         tc_fence_after();
@@ -269,34 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             const uint32_t c_off = (c >> 3) * C::kBlock, cq_off = (c >> 3) * C::kQBlock;
             bool ok = loaders_agree(!*abort_flag);
             unsigned fills = 0, seq = 0, queries = 0;
-            uint32_t waiting[2] = {0u, 0u};                      // barriers of the copies in flight, oldest first
-            int in_flight = 0;
-            auto arrive = [&](uint32_t b) {
-                fence_async_smem();                              // what this thread copied is read by the tensor cores
-                if (b) mbar_arrive(b);
-            };
-            auto flush = [&]() {
-                copies_wait<0>();
-                if (in_flight > 0) arrive(waiting[0]);
-                if (in_flight > 1) arrive(waiting[1]);
-                in_flight = 0;
-            };
-            auto issued = [&](uint32_t b) {                      // copies are under way; their barrier is told two fills later
-                copies_commit();
-                if (in_flight == 2) {
-                    copies_wait<2>();
-                    arrive(waiting[0]);
-                    waiting[0] = waiting[1];
-                    in_flight = 1;
-                }
-                waiting[in_flight++] = b;
-            };
-            auto wait_empty = [&](uint32_t b, uint32_t parity) { // nothing may be held back while this thread waits for the consumers
-                if (ok && !mbar_try_wait(b, parity)) {
-                    flush();
-                    ok = mbar_wait(b, parity, abort_flag, P.wait_budget);
-                }
-            };
+            auto wait_empty = [&](uint32_t b, uint32_t parity) { ok = ok && mbar_wait(b, parity, abort_flag, P.wait_budget); };
             auto fill = [&](const uint16_t* src, const long long* place) {
                 const unsigned s = fills % ST;
                 if (fills >= (unsigned)ST) wait_empty(bar_empty + 8 * s, (fills / ST - 1) & 1);
@@ -307,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         const long long o = place[r];
                         copy16(dst + r * 128 + (((c ^ r) & 7) << 4), o >= 0 ? src + o + c * 8 : q, o >= 0);
                     }
-                    issued(bar_full + 8 * s);
+                    arrive_when_landed(bar_full + 8 * s);
                 }
                 ++fills;
             };
@@ -342,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             const bool here = r < x.rows;
                             copy16(sbase + cq_off + r * 128 + (((c ^ r) & 7) << 4), here ? q + query_offset(A, x, p.h, r) + c * 8 : q, here);
                         }
-                        issued(P.inject == 1 && queries == 0 && lt == 0 ? 0u : bar_q);      // test hook: a barrier that never fills
+                        if (P.inject != 1 || queries > 0 || lt > 0) arrive_when_landed(bar_q);     // test hook: a barrier that never fills
                     }
                     ++queries;
                 };
@@ -373,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 }
                 ok = loaders_agree(ok);                          // the places have been read by everyone
             }
-            flush();
+            copies_wait_all();
         }
     } else {
         // =====================================================================
@@ -469,9 +461,45 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
+                // A tile that every row of the warp sees all of (most of a long context): no masks, and the probabilities stay in
+                // registers until the tile's sum has told that none of them outgrew its maximum.
+                bool stored = false;
+                if ((words[0] & words[1] & words[2] & words[3]) == 0xffffffffu && base + kKeys - 1 <= t_least && t_most - base < A.K &&
+                    !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
+                    uint32_t s[2][32], pk[4][16];
+                    const uint64_t nb2 = pack2(-m, -m);
+                    uint64_t sum0 = 0ull, sum1 = 0ull;
+                    tmem_ld32(scol, s[0]);
+                    landed(s[0]);
 #pragma unroll
-                for (int pc = 0; pc < 4; ++pc) {
+                    for (int pc = 0; pc < 4; ++pc) {
+                        if (pc < 3) tmem_ld32(scol + 32 * (pc + 1), s[(pc + 1) & 1]);
+                        uint32_t(&x)[32] = s[pc & 1];
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const uint64_t e = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, nb2);
+                            const uint64_t g = fma2(pack2(__uint_as_float(x[2 * i + 2]), __uint_as_float(x[2 * i + 3])), sc2, nb2);
+                            const float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e)), c = fast_exp2(lo_of(g)), d = fast_exp2(hi_of(g));
+                            sum0 = add2(sum0, pack2(a, b));
+                            sum1 = add2(sum1, pack2(c, d));
+                            pk[pc][i] = cvt_pack<BF16>(a, b);
+                            pk[pc][i + 1] = cvt_pack<BF16>(c, d);
+                        }
+                        if (pc < 3) landed(s[(pc + 1) & 1]);
+                    }
+                    sum0 = add2(sum0, sum1);
+                    const float rs = lo_of(sum0) + hi_of(sum0);
+                    if (!__any_sync(0xffffffffu, !(rs <= kGrowSum))) {
+                        l += rs;
+                        stored = true;
+#pragma unroll
+                        for (int pc = 0; pc < 4; ++pc) tmem_st16(scol + 16 * pc, pk[pc]);
+                    }
+                }
+#pragma unroll 1
+                for (int pc = stored ? 4 : 0; pc < 4; ++pc) {
                     const int t0 = base + 32 * pc;
+                    const uint32_t word = pc == 0 ? words[0] : pc == 1 ? words[1] : pc == 2 ? words[2] : words[3];
                     uint32_t pk[16];
                     if (t0 > t_most || (t0 + 31 < t_least && t_least - (t0 + 31) >= A.K)) {       // no row of the warp sees the piece
 #pragma unroll
@@ -481,11 +509,11 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     }
                     uint32_t s[32];
                     tmem_ld32(scol + 32 * pc, s);
-                    tmem_ld_wait();
+                    landed(s);
                     // every row of the warp that counts sees all of the piece
-                    const bool open = words[pc] == 0xffffffffu && t0 + 31 <= t_least && t_most - t0 < A.K;
+                    const bool open = word == 0xffffffffu && t0 + 31 <= t_least && t_most - t0 < A.K;
                     uint32_t bits = 0xffffffffu;
-                    if (!open) bits = low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & words[pc];
+                    if (!open) bits = low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & word;
                     bool done = false;
                     if (open && !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
                         const uint64_t nb2 = pack2(-m, -m);
