@@ -98,6 +98,7 @@ bool divide(Args& A, const Shape& shape)
     A.keys = shape.keys;
     A.overhead = shape.overhead;
     A.least = shape.least;
+    A.align = 1;
     const int queries = A.L / A.dil;
     A.long_classes = A.L - queries * A.dil;
     auto tiles = [&](long long n) { return (n * A.G + A.M - 1) / A.M; };

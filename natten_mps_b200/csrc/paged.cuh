@@ -38,6 +38,7 @@ struct Args {
     int pages, page_size, table_width;
     int K, dil;                              // window, at most kAllOfThePast
     int M, keys, overhead, least;            // rows and keys of a tile; in key tiles: what beginning a unit costs, a CTA's least piece
+    int align;                               // tiles start at multiples of it (1 with a dilation)
     int long_classes, tiles_long, tiles_short, per_seq, columns, ctas;
     FastDiv by_page, by_group;
     float scale_log2;                        // scale * log2(e)
@@ -58,7 +59,7 @@ __device__ __forceinline__ float* slot_out(const Args& A, int slot) { return rei
 struct Tile {                                // a row tile of a class of a sequence; the same for every key/value head
     int b, cls, row0, rows;                  // rows: of the class, from row0 on, at most M
     int fresh, t0, residue;                  // new tokens of the sequence; t of the class's first query
-    int lo, hi, n;                           // keys lo ... hi (t), in n tiles
+    int lo, hi, base, n;                     // keys lo ... hi (t), in n tiles from base on
 };
 
 __device__ __forceinline__ Tile tile_of(const Args& A, int column)
@@ -90,7 +91,8 @@ __device__ __forceinline__ Tile tile_of(const Args& A, int column)
     else if (x.hi > (capacity - 1 - x.residue) / A.dil) x.hi = (int)((capacity - 1 - x.residue) / A.dil);
     const int back = x.t0 + first - (A.K - 1);
     x.lo = x.t0 + first > 0 && back > 0 ? back : 0;
-    x.n = last >= first && x.hi >= x.lo ? (x.hi - x.lo) / A.keys + 1 : 0;
+    x.base = x.lo - x.lo % A.align;
+    x.n = last >= first && x.hi >= x.lo ? (x.hi - x.base) / A.keys + 1 : 0;
     return x;
 }
 

@@ -14,9 +14,12 @@
 // which the row sum of a piece tells; O, the sum and the tile's probabilities so far are then rescaled by the thread itself.  So
 // there is no running maximum, and no thread has to touch O in between.
 //
-// Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products.  The rows of a tile lie anywhere
-// in the cache, so the loading threads look them up in the page table, a tile ahead, and copy them 16 bytes at a time
-// (asynchronously, as far ahead as the stages go) into the swizzled layout that the tensor cores read; a row that is not there is zero.
+// Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products.  The loading threads look the keys
+// of a tile up in the page table, a tile ahead.  Where 16 or more keys at a time are adjacent in a page (no dilation, a page
+// size that is a multiple of 16) tiles start at such a run and TMA brings one run of a tile that is there as a whole.  The other
+// tiles (the first and last of a unit, pages of other sizes, dilated keys) are copied row by row, 16 bytes at a time, into the
+// same swizzled layout; a row that is not there is zero, whatever its slot holds.  Row-wise copies of every tile would take 3750
+// cycles a tile, twice what the products need.
 //
 // TMEM columns: S (P over its first half) of the halves at 0 and 128, O at 256 and 384.
 #include "../../include/natten_b200.h"
@@ -68,7 +71,7 @@ template <int DH, bool SPLIT> struct Cfg {
     static constexpr int kOffFlags = kOffBars + 8 * kBars;       // abort flag, TMEM address
     static constexpr int kOffScratch = (kOffFlags + 8 + 15) & ~15;
     static constexpr int kSmem = kOffScratch + 36 * 8;
-    static_assert(kSmem <= kMaxDynamicSmem, "shared memory of a CTA");
+    static_assert(kTile % 1024 == 0 && kSmem <= kMaxDynamicSmem, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
@@ -82,6 +85,22 @@ __device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_
 __device__ __forceinline__ void arrive_when_landed(uint32_t b)
 {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b) : "memory");
+}
+// 2^x of two values on the FMA pipe, for a share of the exponentials (the special-function unit does 16 a cycle, the products of a
+// tile leave it one cycle for each): x = n + f with n the nearest whole number, 2^f by the polynomial of degree 4 with the least
+// largest relative error on [-1/2, 1/2] (2.6e-6, from a Remez exchange), n added to the exponent.  Values above 127 and NaN give 2^127,
+// which the tile's sum tells.
+__device__ __forceinline__ void exp2_fma(uint64_t e, float& a, float& b)
+{
+    const uint64_t x = pack2(fmaxf(fminf(lo_of(e), 127.f), -126.f), fmaxf(fminf(hi_of(e), 127.f), -126.f));
+    constexpr float kRound = 12582912.f;     // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
+    const uint64_t r = add2(x, pack2(kRound, kRound)), n = add2(r, pack2(-kRound, -kRound)), f = fma2(n, pack2(-1.f, -1.f), x);
+    uint64_t y = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, f, pack2(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+    a = __uint_as_float(__float_as_uint(lo_of(y)) + (__float_as_uint(lo_of(r)) << 23));
+    b = __uint_as_float(__float_as_uint(hi_of(y)) + (__float_as_uint(hi_of(r)) << 23));
 }
 // The loads of this thread's TMEM rows have landed: nothing that uses them may move in front of this.
 __device__ __forceinline__ void landed(uint32_t (&r)[32])
@@ -102,7 +121,8 @@ __device__ __forceinline__ bool loaders_agree(bool ok)
 }
 
 template <int DH, bool BF16, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Args A, const __grid_constant__ Status P)
+__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Args A,
+          const __grid_constant__ Status P)
 {
     using C = Cfg<DH, SPLIT>;
     constexpr int ST = C::kStages;
@@ -289,42 +309,61 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             bool ok = loaders_agree(!*abort_flag);
             unsigned fills = 0, seq = 0, queries = 0;
             auto wait_empty = [&](uint32_t b, uint32_t parity) { ok = ok && mbar_wait(b, parity, abort_flag, P.wait_budget); };
-            auto fill = [&](const uint16_t* src, const long long* place) {
-                const unsigned s = fills % ST;
-                if (fills >= (unsigned)ST) wait_empty(bar_empty + 8 * s, (fills / ST - 1) & 1);
-                if (ok) {
-                    const uint32_t dst = sbase + C::kOffKV + s * C::kTile + c_off;
-#pragma unroll 4
-                    for (int r = r0; r < kKeys; r += kAtOnce) {
-                        const long long o = place[r];
-                        copy16(dst + r * 128 + (((c ^ r) & 7) << 4), o >= 0 ? src + o + c * 8 : q, o >= 0);
-                    }
-                    arrive_when_landed(bar_full + 8 * s);
-                }
-                ++fills;
-            };
+            // A tile's keys: this thread's (the lt-th) page and slot, and where the keys and values of all of them are (elements).
+            // whole: every key is there, and they come in runs of A.align.
+            struct Keys { int page, slot; bool whole; const long long* at; };
             for (; ok && piece.more(); piece.advance(A)) {
                 const Piece::Portion p = piece.portion(A);
                 if (!p.work) continue;
                 const Tile& x = piece.tile;
                 const int n = p.x1 - p.x0;
+                auto fill = [&](const CUtensorMap* map, const uint16_t* src, const Keys& k, int offset) {
+                    const unsigned s = fills % ST;
+                    const uint32_t full = bar_full + 8 * s, dst = sbase + C::kOffKV + s * C::kTile;
+                    if (fills >= (unsigned)ST) wait_empty(bar_empty + 8 * s, (fills / ST - 1) & 1);
+                    if (ok && k.whole) {
+                        if (lt == 0) mbar_expect_tx(full, C::kTile);
+                        else mbar_arrive(full);
+                        if ((lt & (A.align - 1)) == 0)
+#pragma unroll
+                            for (int b = 0; b < C::kBlocks; ++b)
+                                tma_load_5d(dst + b * C::kBlock + lt * 128, map, full, 0, k.slot, b, p.h, k.page);
+                    } else if (ok) {
+#pragma unroll 4
+                        for (int r = r0; r < kKeys; r += kAtOnce) {
+                            const long long o = k.at[offset + r];
+                            copy16(dst + c_off + r * 128 + (((c ^ r) & 7) << 4), o >= 0 ? src + o + c * 8 : q, o >= 0);
+                        }
+                        arrive_when_landed(full);
+                    }
+                    ++fills;
+                };
                 int page = 0, slot = 0;
-                bool there = locate(A, x, x.lo + p.x0 * kKeys + lt, page, slot);
-                // Places of tile j (the lookup for the next one is under way while this one is copied).  Three buffers: with kSplit
-                // a thread may still copy the values of tile j - 2 when another writes the places of tile j.
-                auto place_tile = [&](int j) {
-                    long long* at = places + (j % 3) * 2 * kKeys;
-                    at[lt] = there ? page * A.ks[0] + slot * A.ks[1] + p.h * A.ks[2] : -1;
-                    at[kKeys + lt] = there ? page * A.vs[0] + slot * A.vs[1] + p.h * A.vs[2] : -1;
+                bool there = false;
+                auto look_up = [&](int j) {
+                    const int t = x.base + (p.x0 + j) * kKeys + lt;
+                    there = j < n && t >= x.lo && locate(A, x, t, page, slot);
+                };
+                look_up(0);
+                // Tile j (the lookup for the next one is under way while this one is copied).  Three buffers: with kSplit a thread
+                // may still copy the values of tile j - 2 when another writes the places of tile j.
+                auto keys_of = [&](int j) {
+                    Keys k{page, slot, false, places + (j % 3) * 2 * kKeys};
                     const unsigned seen = __ballot_sync(0xffffffffu, there), w = seq % kWordSlots;
                     if (lane == 0) {
                         reinterpret_cast<unsigned*>(smem + C::kOffWords)[4 * w + (warp & 3)] = seen;
                         mbar_arrive(bar_words + 8 * w);
                     }
                     ++seq;
-                    there = j + 1 < n && locate(A, x, x.lo + (p.x0 + j + 1) * kKeys + lt, page, slot);
+                    if (A.align > 1) k.whole = loaders_agree(there);
+                    if (!k.whole) {
+                        long long* at = places + (j % 3) * 2 * kKeys;
+                        at[lt] = there ? page * A.ks[0] + slot * A.ks[1] + p.h * A.ks[2] : -1;
+                        at[kKeys + lt] = there ? page * A.vs[0] + slot * A.vs[1] + p.h * A.vs[2] : -1;
+                    }
+                    look_up(j + 1);
                     ok = loaders_agree(ok);
-                    return at;
+                    return k;
                 };
                 auto load_queries = [&]() {
                     if (queries > 0) wait_empty(bar_qfree, (queries - 1) & 1);
@@ -338,28 +377,26 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     }
                     ++queries;
                 };
-                const long long* at = place_tile(0);
+                Keys k = keys_of(0);
                 if (!ok) break;
-                fill(kc, at);
+                fill(&tmK, kc, k, 0);
                 load_queries();
-                if constexpr (SPLIT) {
-                    for (int j = 0; j < n; ++j) {
-                        const long long* next = nullptr;
+                for (int j = 0; j < n; ++j) {
+                    if constexpr (SPLIT) {                       // K0, K1, V0, K2, V1, ...
+                        Keys next{};
                         if (j + 1 < n) {
-                            next = place_tile(j + 1);
+                            next = keys_of(j + 1);
                             if (!ok) break;
-                            fill(kc, next);
+                            fill(&tmK, kc, next, 0);
                         }
-                        fill(vc, at + kKeys);
-                        at = next;
-                    }
-                } else {
-                    for (int j = 0; j < n; ++j) {
-                        fill(vc, at + kKeys);
+                        fill(&tmV, vc, k, kKeys);
+                        k = next;
+                    } else {                                     // K0, V0, K1, V1, ...
+                        fill(&tmV, vc, k, kKeys);
                         if (j + 1 < n) {
-                            at = place_tile(j + 1);
+                            k = keys_of(j + 1);
                             if (!ok) break;
-                            fill(kc, at);
+                            fill(&tmK, kc, k, 0);
                         }
                     }
                 }
@@ -451,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             bool had_tiles = false;
             for (int j = 0; j < n; ++j, ++seq) {
                 if (SPLIT && (j & 1) != half) continue;
-                const int base = x.lo + (p.x0 + j) * kKeys;
+                const int base = x.base + (p.x0 + j) * kKeys;
                 const unsigned w = seq % kWordSlots;
                 ok = ok && mbar_wait(bar_words + 8 * w, (seq / kWordSlots) & 1, abort_flag, P.wait_budget);
                 const volatile uint32_t* there_words = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffWords) + 4 * w;
@@ -479,7 +516,13 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         for (int i = 0; i < 16; i += 2) {
                             const uint64_t e = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, nb2);
                             const uint64_t g = fma2(pack2(__uint_as_float(x[2 * i + 2]), __uint_as_float(x[2 * i + 3])), sc2, nb2);
-                            const float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e)), c = fast_exp2(lo_of(g)), d = fast_exp2(hi_of(g));
+                            float a = 0.f, b = 0.f;
+                            if (i % 6 == 0) exp2_fma(e, a, b);
+                            else {
+                                a = fast_exp2(lo_of(e));
+                                b = fast_exp2(hi_of(e));
+                            }
+                            const float c = fast_exp2(lo_of(g)), d = fast_exp2(hi_of(g));
                             sum0 = add2(sum0, pack2(a, b));
                             sum1 = add2(sum1, pack2(c, d));
                             pk[pc][i] = cvt_pack<BF16>(a, b);
@@ -514,31 +557,37 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     const bool open = word == 0xffffffffu && t0 + 31 <= t_least && t_most - t0 < A.K;
                     uint32_t bits = 0xffffffffu;
                     if (!open) bits = low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & word;
+                    if (__any_sync(0xffffffffu, m == -CUDART_INF_F && bits != 0u)) {         // first columns that a row sees
+                        float top = -CUDART_INF_F;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * A.scale_log2);
+                        if (m == -CUDART_INF_F) m = top;
+                    }
                     bool done = false;
-                    if (open && !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
-                        const uint64_t nb2 = pack2(-m, -m);
-                        uint64_t sum = 0ull;
+                    {
+                        const float shift = m == -CUDART_INF_F ? 0.f : -m;
+                        const uint64_t nb2 = pack2(shift, shift);
+                        float sum_a = 0.f, sum_b = 0.f;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const uint64_t e = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, nb2);
-                            const float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e));
-                            sum = add2(sum, pack2(a, b));
+                            float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e));
+                            if (!open) {                         // whatever a hidden score gave
+                                a = (bits >> (2 * i)) & 1u ? a : 0.f;
+                                b = (bits >> (2 * i + 1)) & 1u ? b : 0.f;
+                            }
+                            sum_a += a;
+                            sum_b += b;
                             pk[i] = cvt_pack<BF16>(a, b);
                         }
-                        const float rs = lo_of(sum) + hi_of(sum);
+                        const float rs = sum_a + sum_b;
                         if (!__any_sync(0xffffffffu, !(rs <= kGrowSum))) {
                             l += rs;
                             done = true;
                         }
                     }
                     if (!done) {
-                        if (m == -CUDART_INF_F && bits != 0u) {  // first columns that the row sees
-                            float top = -CUDART_INF_F;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * A.scale_log2);
-                            m = top;
-                        }
                         const float base_m = m == -CUDART_INF_F ? 0.f : m;
                         float over = -CUDART_INF_F;
 #pragma unroll
@@ -612,12 +661,12 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 4; ++i) rows4[i] = __shfl_sync(0xffffffffu, my_row, (lane & ~3) | i);
             const int piece4 = lane & 3;
-#pragma unroll 1
+#pragma unroll
             for (int part = 0; part < DH / 32; ++part) {
                 uint32_t o[32];
                 if (n > 0) {
                     tmem_ld32(ocol + 32 * part, o);
-                    tmem_ld_wait();
+                    landed(o);
                     if (both) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -686,6 +735,15 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 
 } // namespace
 
+// Keys of a cache, 64 channels of one head: [64, slot, block of 64 channels, head, page]; a box is `run` slots.
+static bool encode_cache(CUtensorMap* map, const Args& A, bool bf16, const void* cache, const int64_t (&strides)[3], int run)
+{
+    const cuuint64_t dims[5] = {64, (cuuint64_t)A.page_size, (cuuint64_t)A.D / 64, (cuuint64_t)A.Hkv, (cuuint64_t)A.pages};
+    const cuuint64_t bytes[4] = {(cuuint64_t)strides[1] * 2, 128, (cuuint64_t)strides[2] * 2, (cuuint64_t)strides[0] * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)run, 1, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
+    return tcplan::encode_16bit(map, cache, bf16, dims, bytes, box, steps);
+}
+
 bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape)
 {
     if ((dtype != NATTEN_F16 && dtype != NATTEN_BF16) || !aligned || (A.D != 64 && A.D != 128)) return false;
@@ -695,20 +753,27 @@ bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape)
     return true;
 }
 
-int tc_run(int dtype, const Args& A, cudaStream_t s)
+int tc_run(int dtype, const Args& call, cudaStream_t s)
 {
+    Args A = call;
     Status st{};
     st.wait_budget = tcplan::debug_wait_budget();
     st.inject = tcplan::debug_inject();
     cudaError_t err = tcplan::status_ptr(st.status);
     if (err == cudaSuccess) err = tcplan::status_host_ptr(st.status_host);
     if (err != cudaSuccess) return (int)err;
+    // Runs of 64, 32 or 16 adjacent keys where the page size is a multiple of that many and nothing is dilated.
+    CUtensorMap mk{}, mv{};
+    if (A.dil == 1 && A.pages > 0 && A.page_size % 16 == 0) {
+        const int run = A.page_size % 64 == 0 ? 64 : A.page_size % 32 == 0 ? 32 : 16;
+        if (encode_cache(&mk, A, dtype == NATTEN_BF16, A.kc, A.ks, run) && encode_cache(&mv, A, dtype == NATTEN_BF16, A.vc, A.vs, run)) A.align = run;
+    }
     auto go = [&](auto dh, auto bf, auto split) {
         constexpr int kDim = decltype(dh)::value;
         using C = Cfg<kDim, decltype(split)::value>;
         auto* kernel = tc_kernel<kDim, decltype(bf)::value, decltype(split)::value>;
         err = ensure_dynamic_smem((const void*)kernel, C::kSmem);
-        if (err == cudaSuccess) kernel<<<A.ctas, kThreads, C::kSmem, s>>>(A, st);
+        if (err == cudaSuccess) kernel<<<A.ctas, kThreads, C::kSmem, s>>>(mk, mv, A, st);
     };
     auto by_rows = [&](auto dh, auto bf) {
         if (A.M == kHalfRows) go(dh, bf, std::true_type{});

@@ -254,3 +254,18 @@ def test_paths():
             path(BF16, 1, 16, 4, 128)
     finally:
         _cabi.set_force(None)
+
+
+@pytest.mark.parametrize("kernel", [None, 150])
+@pytest.mark.parametrize("page,D", [(16, 64), (64, 128), (32, 128), (24, 64)])
+@pytest.mark.parametrize("L,Hq,Hkv", [(1, 4, 2), (70, 8, 2), (40, 4, 2)], ids=["warp", "rows", "split_keys"])
+def test_missing_pages(L, Hq, Hkv, page, D, kernel):
+    """Holes in the page table and slots that no token was written to, NaN in all of them, in the middle of tiles."""
+    q, k_cache, v_cache, table, lens, new = _problem(BF16, [700, 333], [L, L - L // 3], L, Hq, Hkv, D, page)
+    for b, slots in ((0, (0, 3, 5)), (1, (1, table.shape[1] - 1, 333 // page))):
+        for n in slots:
+            k_cache[table[b, n]] = math.nan
+            v_cache[table[b, n]] = math.nan
+            table[b, n] = (-1, 10 ** 9)[n % 2]
+    out, _ = _check((q, k_cache, v_cache, table, lens, new), kernel, 1)
+    assert not bool(out.isnan().any())
