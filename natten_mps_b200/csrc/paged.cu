@@ -11,84 +11,165 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace natten {
 namespace paged {
 namespace {
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinWarps = 8, kJoinThreads = 32 * kJoinWarps;
 
 template <typename T> __device__ __forceinline__ T rounded(float x);
 template <> __device__ __forceinline__ float rounded(float x) { return x; }
 template <> __device__ __forceinline__ __half rounded(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 rounded(float x) { return __float2bfloat16_rn(x); }
 
-// Block (c, y): rows y * 4 ... of the unit that CTA c's piece ends inside of, a row a warp.  Its parts are in slot 2c + 1 and in
-// slots 2(c + 1), 2(c + 2), ... up to the CTA that finishes the unit.  With M = max m_i: sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-template <typename T> __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args A)
+// Block (c, y): rows y * ROWS ... of the unit that CTA c began and others went on with.  With M = max m_i its rows are
+// sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the parts i.  Warps take a row each; where a block has fewer rows than warps
+// several share a row's parts.  A lane holds four channels of every 128, and asks for several parts at a time: what this costs is
+// the latency of the workspace, so everything that does not depend on an answer is asked for at once.
+template <typename T, int ROWS, int DC> __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args A)
 {
-    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Shared* all = reinterpret_cast<const Shared*>(A.ws);
-    const int unit = all[c].tail;
-    if (unit < 0) return;
-    const int column = unit / A.Hkv, h = unit - column * A.Hkv;
+    constexpr int kShare = ROWS >= kJoinWarps ? 1 : kJoinWarps / ROWS;   // warps of a row
+    constexpr int kAtOnce = 8 / DC;                                      // parts asked for at a time
+    __shared__ float4 others[kJoinWarps][32 * DC];
+    __shared__ float other_sums[kJoinWarps];
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % kShare;
+    wait_for_primary();
+    const Shared mine = reinterpret_cast<const Shared*>(A.ws)[c];
+    if (mine.unit < 0) return;
+    const int column = mine.unit / A.Hkv, h = mine.unit - column * A.Hkv, parts = mine.parts;
     const Tile x = tile_of(A, column);
-    const int row = blockIdx.y * (kJoinThreads / 32) + warp;
-    if (row >= x.rows) return;
-    int parts = 1;                           // CTAs of the unit
-    for (bool on = true; on;) {
-        const int k = c + parts + lane;
-        const bool part = k < A.ctas && all[k].head == unit;
-        const unsigned ends = __ballot_sync(0xffffffffu, !part || all[k].head_done);
-        if (ends) {
-            const int e = __ffs(ends) - 1;
-            parts += e + (__shfl_sync(0xffffffffu, (int)part, e) ? 1 : 0);
-            on = false;
-        } else {
-            parts += 32;
-        }
-    }
     auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
-    float top = -CUDART_INF_F;
-    bool bad = false;                        // a NaN maximum
-    for (int i = lane; i < parts; i += 32) {
-        const float m = slot_sums(A, slot(i))[row].x;
-        bad = bad || m != m;
-        top = fmaxf(top, m);
+    for (int r = warp / kShare; r < ROWS; r += kJoinWarps / kShare) {    // as many rounds in every warp of the block
+        const int row = blockIdx.y * ROWS + r;
+        const bool real = row < x.rows;
+        float top = -CUDART_INF_F;
+        bool bad = false;
+        if (real)
+            for (int i = lane; i < parts; i += 32) {
+                const float m = slot_sums(A, slot(i))[row].x;
+                bad = bad || m != m;
+                top = fmaxf(top, m);
+            }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (__any_sync(0xffffffffu, bad)) top = CUDART_NAN_F;
+        const float base = top == -CUDART_INF_F ? 0.f : top;
+        float total = 0.f;
+        float4 acc[DC];
+#pragma unroll
+        for (int d = 0; d < DC; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (real)
+            for (int i0 = share; i0 < parts; i0 += kShare * kAtOnce) {
+                float2 ml[kAtOnce];
+                float4 o[kAtOnce][DC];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const int i = i0 + k * kShare;
+                    ml[k] = make_float2(-CUDART_INF_F, 0.f);
+                    if (i >= parts) continue;
+                    ml[k] = slot_sums(A, slot(i))[row];
+                    const float* src = slot_out(A, slot(i)) + (long long)row * A.D;
+#pragma unroll
+                    for (int d = 0; d < DC; ++d) {
+                        const int ch = 128 * d + 4 * lane;
+                        o[k][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (A.D % 4 == 0) {
+                            if (ch < A.D) o[k][d] = *reinterpret_cast<const float4*>(src + ch);
+                        } else {
+                            if (ch < A.D) o[k][d].x = src[ch];
+                            if (ch + 1 < A.D) o[k][d].y = src[ch + 1];
+                            if (ch + 2 < A.D) o[k][d].z = src[ch + 2];
+                            if (ch + 3 < A.D) o[k][d].w = src[ch + 3];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const float f = exp2f(ml[k].x - base);
+                    if (f == 0.f) continue;                              // a part that saw nothing
+                    total = fmaf(f, ml[k].y, total);
+#pragma unroll
+                    for (int d = 0; d < DC; ++d) {
+                        acc[d].x = fmaf(f, o[k][d].x, acc[d].x);
+                        acc[d].y = fmaf(f, o[k][d].y, acc[d].y);
+                        acc[d].z = fmaf(f, o[k][d].z, acc[d].z);
+                        acc[d].w = fmaf(f, o[k][d].w, acc[d].w);
+                    }
+                }
+            }
+        if constexpr (kShare > 1) {
+            __syncthreads();                                             // the last round's have been read
+#pragma unroll
+            for (int d = 0; d < DC; ++d) others[warp][32 * d + lane] = acc[d];
+            if (lane == 0) other_sums[warp] = total;
+            __syncthreads();
+            if (share == 0) {
+#pragma unroll
+                for (int k = 1; k < kShare; ++k) {
+                    total += other_sums[warp + k];
+#pragma unroll
+                    for (int d = 0; d < DC; ++d) {
+                        const float4 y = others[warp + k][32 * d + lane];
+                        acc[d].x += y.x;
+                        acc[d].y += y.y;
+                        acc[d].z += y.z;
+                        acc[d].w += y.w;
+                    }
+                }
+            }
+        }
+        if (!real || share != 0) continue;
+        long long index;
+        int t;
+        const bool live = row_of(A, x, h, row, index, t);
+        const bool some = live && total != 0.f;                          // (a NaN stays one)
+        const float inv = some ? 1.f / total : 0.f;
+#pragma unroll
+        for (int d = 0; d < DC; ++d) {
+            const float y[4] = {acc[d].x, acc[d].y, acc[d].z, acc[d].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int ch = 128 * d + 4 * lane + e;
+                if (ch < A.D) static_cast<T*>(A.out)[index * A.D + ch] = rounded<T>(some ? y[e] * inv : 0.f);
+            }
+        }
+        if (A.lse && lane == 0) A.lse[index] = some ? (base + log2f(total)) * 0.6931471805599453f : -CUDART_INF_F;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (__any_sync(0xffffffffu, bad)) top = CUDART_NAN_F;
-    const float base = top == -CUDART_INF_F ? 0.f : top;
-    float total = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = slot_sums(A, slot(i))[row];
-        const float f = exp2f(ml.x - base);
-        total = fmaf(f, ml.y, total);
-        if (f == 0.f) continue;              // a part that saw nothing
-        const float* o = slot_out(A, slot(i)) + (long long)row * A.D;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < A.D) acc[e] = fmaf(f, o[lane + 32 * e], acc[e]);
-    }
-    long long index;
-    int t;
-    row_of(A, x, h, row, index, t);
-    const float inv = total > 0.f ? 1.f / total : total;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (lane + 32 * e < A.D) static_cast<T*>(A.out)[index * A.D + lane + 32 * e] = rounded<T>(acc[e] * inv);
-    if (A.lse && lane == 0) A.lse[index] = total == 0.f ? -CUDART_INF_F : (base + log2f(total)) * 0.6931471805599453f;
 }
 
+// The joining kernel starts while the last CTAs of the kernel in front of it are still at work, and waits for their results.
 int join(int dtype, const Args& A, cudaStream_t s)
 {
-    const dim3 grid(A.ctas, (A.M + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
-    if (dtype == NATTEN_F32) join_kernel<float><<<grid, kJoinThreads, 0, s>>>(A);
-    else if (dtype == NATTEN_F16) join_kernel<__half><<<grid, kJoinThreads, 0, s>>>(A);
-    else join_kernel<__nv_bfloat16><<<grid, kJoinThreads, 0, s>>>(A);
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cudaError_t err = cudaSuccess;
+    auto go = [&](auto type, auto rows, auto dc) {
+        constexpr int kRows = decltype(rows)::value;
+        cfg.gridDim = dim3(A.ctas, (A.M + kRows - 1) / kRows);
+        err = cudaLaunchKernelEx(&cfg, join_kernel<decltype(type), kRows, decltype(dc)::value>, A);
+    };
+    // Many rows: a block for 32 of them.  Few rows may have a part in every CTA: two rows a block, four warps each.
+    auto by_rows = [&](auto type, auto dc) {
+        if (A.M > 32) go(type, std::integral_constant<int, 32>{}, dc);
+        else go(type, std::integral_constant<int, 2>{}, dc);
+    };
+    auto by_dim = [&](auto type) {
+        if (A.D <= 128) by_rows(type, std::integral_constant<int, 1>{});
+        else by_rows(type, std::integral_constant<int, 2>{});
+    };
+    if (dtype == NATTEN_F32) by_dim(float{});
+    else if (dtype == NATTEN_F16) by_dim(__half{});
+    else by_dim(__nv_bfloat16{});
     simt_count_launch(1);
-    return (int)cudaGetLastError();
+    return (int)err;
 }
 
 // Tile counts of the padded batch, whatever the lengths are.  False: more units than 31 bits number.
@@ -99,6 +180,10 @@ bool divide(Args& A, const Shape& shape)
     A.overhead = shape.overhead;
     A.least = shape.least;
     A.align = 1;
+    // tiles that the keys of a unit can have: a window and the queries behind its first, what the table can hold
+    const long long held = (long long)A.table_width * A.page_size / A.dil + 1;
+    const long long reach = std::min(held, (long long)A.K + (A.M + A.G - 1) / A.G);
+    A.whole = reach <= (long long)(shape.most - 1) * shape.keys;
     const int queries = A.L / A.dil;
     A.long_classes = A.L - queries * A.dil;
     auto tiles = [&](long long n) { return (n * A.G + A.M - 1) / A.M; };
@@ -195,7 +280,7 @@ int natten_paged_fwd(const natten_paged_params_t* p, const void* q, const void* 
     note_path(c.family == Family::kTc ? NATTEN_PATH_TCGEN05 : c.family == Family::kWarp ? NATTEN_PATH_WARP : NATTEN_PATH_SIMT);
     const int err = c.family == Family::kTc ? tc_run(p->dtype, A, s) : c.family == Family::kWarp ? warp_run(p->dtype, A, s)
                                                                                                : general_run(p->dtype, A, c.aligned, s);
-    return err ? err : join(p->dtype, A, s);
+    return err || A.whole ? err : join(p->dtype, A, s);
 }
 
 } // extern "C"

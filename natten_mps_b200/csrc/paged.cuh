@@ -15,6 +15,8 @@
 // with no host read and no atomics.  A unit that lies inside one piece is written out directly.  Of one that several CTAs share,
 // each writes its unnormalised sum, maximum and row sum to the workspace (at most two units a CTA: one that its piece begins
 // inside of, one that it ends inside of), and a second kernel joins them, in the CTAs' order: results do not depend on timing.
+// Where windows or tables keep every unit short (`whole`), a CTA takes the units that begin in its piece, to their ends: the
+// second kernel and the partial results would cost more than the unequal shares.
 #pragma once
 #include "fast_div.cuh"
 
@@ -38,17 +40,18 @@ struct Args {
     int pages, page_size, table_width;
     int K, dil;                              // window, at most kAllOfThePast
     int M, keys, overhead, least;            // rows and keys of a tile; in key tiles: what beginning a unit costs, a CTA's least piece
+    int whole;                               // units are not shared
     int align;                               // tiles start at multiples of it (1 with a dilation)
     int long_classes, tiles_long, tiles_short, per_seq, columns, ctas;
     FastDiv by_page, by_group;
     float scale_log2;                        // scale * log2(e)
 };
 
-// What a CTA tells the joining kernel: the unit that its piece ends inside of (its slot 2c + 1), the one that it begins inside of
-// (slot 2c), and whether it finishes that one.  -1: none.
-struct Shared { int tail, head, head_done, pad; };
+// What a CTA tells the joining kernel: the unit that it began and others go on with (-1: none), and how many CTAs share it.  Its
+// own part of it is in its slot 2c + 1, the next ones' in 2(c + 1), 2(c + 2), ...
+struct Shared { int unit, parts; };
 
-__host__ __device__ inline size_t shared_bytes(int ctas) { return (size_t)ctas * sizeof(Shared); }
+__host__ __device__ inline size_t shared_bytes(int ctas) { return ((size_t)ctas * sizeof(Shared) + 15) & ~(size_t)15; }
 __host__ __device__ inline size_t slot_bytes(int M, int D) { return (size_t)M * (D + 2) * sizeof(float); }
 __device__ __forceinline__ float2* slot_sums(const Args& A, int slot)     // [M] maximum (of scale * log2(e) * score), row sum
 {
@@ -98,8 +101,8 @@ __device__ __forceinline__ Tile tile_of(const Args& A, int column)
 
 // A CTA's piece, unit by unit.  `begin` is called by all `kThreads` threads; the rest is uniform arithmetic.
 struct Piece {
-    long long left;
-    int column, h, off;                      // where the piece goes on: unit (column, h), cost `off` into it
+    long long left, share, rest;             // the first `pieces` CTAs have `share` each, and the rest among them
+    int pieces, column, h, off;              // where the piece goes on: unit (column, h), cost `off` into it
     Tile tile;
 
     // portion of the unit (column, h): key tiles [x0, x1).  n == 0: nothing to see, rows are to be cleared if `first`.
@@ -131,8 +134,10 @@ struct Piece {
         const long long from = before + upto - mine;
         // no CTA gets less than `least`: every piece of a unit then has tiles, and a unit's CTAs are consecutive
         const int n = (int)min((long long)A.ctas, max(total / A.least, 1ll));
-        const long long share = total / n, rest = total - share * n;       // total * cta / n without overflow
-        const long long start = cta < n ? share * cta + rest * cta / n : total, stop = cta < n ? share * (cta + 1) + rest * (cta + 1) / n : total;
+        pieces = n;
+        share = total / n;
+        rest = total - share * n;
+        const long long start = start_of(cta), stop = start_of(cta + 1);
         if (start >= from && start < from + mine) {
             long long at = start - from;
             int c = c0;
@@ -153,17 +158,28 @@ struct Piece {
             const int w = tile.n + A.overhead;
             h = (int)(found[1] / w);
             off = (int)(found[1] - (long long)h * w);
+            if (A.whole && off > 0) advance(A);              // another CTA's
         }
     }
+    // where CTA c's piece starts: total * c / pieces, without overflow
+    __device__ __forceinline__ long long start_of(int c) const { return c < pieces ? share * c + rest * c / pieces : share * pieces + rest; }
+    // CTAs from `cta` on that share the unit that its piece ends inside of
+    __device__ int parts(const Args& A, int cta) const
+    {
+        const long long end = start_of(cta + 1) + (tile.n + A.overhead - off - left);
+        int c = cta + 1;
+        if (share > 0) c = max(c, (int)min((long long)pieces, end / (share + 1)));    // start_of(c) <= (share + 1) c
+        while (c < pieces && start_of(c) < end) ++c;
+        return c - cta;
+    }
+    __device__ __forceinline__ int take(const Args& A, int w) const { return A.whole || left >= w - off ? w - off : (int)left; }
     __device__ __forceinline__ bool more() const { return left > 0; }
     __device__ __forceinline__ Portion portion(const Args& A) const
     {
         Portion p;
-        const int w = tile.n + A.overhead;
-        const int take = left < w - off ? (int)left : w - off;
         p.h = h;
         p.x0 = max(off - A.overhead, 0);
-        p.x1 = max(off + take - A.overhead, 0);
+        p.x1 = max(off + take(A, tile.n + A.overhead) - A.overhead, 0);
         p.first = off == 0;
         p.work = p.x1 > p.x0;
         p.whole = p.work && p.x0 == 0 && p.x1 == tile.n;
@@ -171,10 +187,9 @@ struct Piece {
     }
     __device__ __forceinline__ void advance(const Args& A)
     {
-        const int w = tile.n + A.overhead;
-        const int take = left < w - off ? (int)left : w - off;
-        left -= take;
-        off += take;
+        const int w = tile.n + A.overhead, t = take(A, w);
+        left -= t;
+        off += t;
         if (off == w) {
             off = 0;
             if (++h == A.Hkv) {
@@ -212,13 +227,19 @@ __device__ __forceinline__ bool locate(const Args& A, const Tile& x, int t, int&
 
 // Host side.  A kernel family says which tiles it would use (false: it does not cover the call); `plan` divides the call by
 // them.  `aligned`: every row of q and of the caches starts on a 16-byte boundary.
-struct Shape { int M, keys, overhead, least, ctas; };
+// most: key tiles up to which a unit is not shared
+struct Shape { int M, keys, overhead, least, most, ctas; };
 bool general_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int general_run(int dtype, const Args& A, bool aligned, cudaStream_t s);
 bool warp_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int warp_run(int dtype, const Args& A, cudaStream_t s);
 bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int tc_run(int dtype, const Args& A, cudaStream_t s);
+
+// A kernel that others may start behind: its dependents' launch overlaps its end.
+__device__ __forceinline__ void let_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Everything that the kernel in front wrote is there.
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 } // namespace paged
 

@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant
 
     Piece piece;
     piece.begin<kThreads>(A, blockIdx.x, scratch);
-    Shared told{-1, -1, 0, 0};
+    let_dependents_launch();
+    Shared told{-1, 0};
     for (; piece.more(); piece.advance(A)) {
         const Piece::Portion p = piece.portion(A);
         const Tile& x = piece.tile;
@@ -178,14 +179,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant
 
         const bool direct = clear || p.whole;
         const int slot = 2 * (int)blockIdx.x + (p.x0 == 0 ? 1 : 0);
-        if (!direct) {
-            const int unit = piece.column * A.Hkv + p.h;
-            if (p.x0 == 0) told.tail = unit;
-            else {
-                told.head = unit;
-                told.head_done = p.x1 == x.n;
-            }
-        }
+        if (!direct && p.x0 == 0) told = {piece.column * A.Hkv + p.h, piece.parts(A, blockIdx.x)};
 #pragma unroll
         for (int r = 0; r < kPerWarp; ++r) {
             const int row = warp * kPerWarp + r;
@@ -213,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant
 bool general_shape(int dtype, const Args& A, bool, Shape& shape)
 {
     if (dtype != NATTEN_F32 && dtype != NATTEN_F16 && dtype != NATTEN_BF16) return false;
-    shape = {kRows, kKeys, 1, 1, 3 * sm_count()};
+    shape = {kRows, kKeys, 1, 1, 16, 3 * sm_count()};
     return A.D <= 256;
 }
 

@@ -170,11 +170,12 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     }
     Piece piece;
     piece.begin<kThreads>(A, blockIdx.x, smem + C::kOffScratch);
+    let_dependents_launch();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    Shared told{-1, -1, 0, 0};
+    Shared told{-1, 0};
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
@@ -425,14 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             const int n = p.work ? p.x1 - p.x0 : 0;
             const bool direct = clear || p.whole;
             const int where = 2 * (int)blockIdx.x + (p.x0 == 0 ? 1 : 0);
-            if (!direct) {
-                const int unit = piece.column * A.Hkv + p.h;
-                if (p.x0 == 0) told.tail = unit;
-                else {
-                    told.head = unit;
-                    told.head_done = p.x1 == x.n;
-                }
-            }
+            if (!direct && p.x0 == 0) told = {piece.column * A.Hkv + p.h, piece.parts(A, blockIdx.x)};
             const bool active = SPLIT ? half == 0 || n > 1 : half == 0 || x.rows > kHalfRows;
             if (!active) {
                 seq += n;
@@ -749,7 +743,7 @@ bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape)
     if ((dtype != NATTEN_F16 && dtype != NATTEN_BF16) || !aligned || (A.D != 64 && A.D != 128)) return false;
     const long long rows = ((long long)A.L + A.dil - 1) / A.dil * A.G;
     if (rows <= 32) return false;
-    shape = {rows > kHalfRows ? 2 * kHalfRows : kHalfRows, kKeys, 1, 2, sm_count()};
+    shape = {rows > kHalfRows ? 2 * kHalfRows : kHalfRows, kKeys, 1, 2, 8, sm_count()};
     return true;
 }
 

@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, MT>::kPerSm) warp_kernel(con
 
     Piece piece;
     piece.begin<kThreads>(A, blockIdx.x, scratch);
-    Shared told{-1, -1, 0, 0};
+    let_dependents_launch();
+    Shared told{-1, 0};
     for (; piece.more(); piece.advance(A)) {
         const Piece::Portion p = piece.portion(A);
         const Tile& x = piece.tile;
@@ -272,14 +273,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, MT>::kPerSm) warp_kernel(con
         __syncthreads();
         const bool direct = clear || p.whole;
         const int where = 2 * (int)blockIdx.x + (p.x0 == 0 ? 1 : 0);
-        if (!direct) {
-            const int unit = piece.column * A.Hkv + p.h;
-            if (p.x0 == 0) told.tail = unit;
-            else {
-                told.head = unit;
-                told.head_done = p.x1 == x.n;
-            }
-        }
+        if (!direct && p.x0 == 0) told = {piece.column * A.Hkv + p.h, piece.parts(A, blockIdx.x)};
         const int chunks = A.D / 8;
         for (int e = tid; e < x.rows * chunks; e += kThreads) {
             const int r = e / chunks, c = e - r * chunks;
@@ -354,6 +348,7 @@ bool warp_shape(int dtype, const Args& A, bool aligned, Shape& shape)
     });
     shape.overhead = 1;
     shape.least = 2;
+    shape.most = 16;
     return true;
 }
 
