@@ -196,6 +196,12 @@ bool divide(Args& A, const Shape& shape)
     A.columns = (int)(per * A.B);
     A.ctas = shape.ctas;
     A.by_group = FastDiv((uint32_t)A.G);
+    A.by_dil = FastDiv((uint32_t)A.dil);
+    A.by_seq = FastDiv((uint32_t)std::max(1, A.per_seq));
+    A.by_long = FastDiv((uint32_t)std::max(1, A.tiles_long));
+    A.by_short = FastDiv((uint32_t)std::max(1, A.tiles_short));
+    A.capacity = (int)std::min<long long>((long long)A.table_width * A.page_size, kAllOfThePast);
+    for (A.keys_log = 0; (1 << A.keys_log) < A.keys;) ++A.keys_log;
     return true;
 }
 
@@ -210,7 +216,7 @@ int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void*
         p->pages < 0 || p->page_size <= 0 || p->table_width < 0 || p->kernel < 0 || p->dilation <= 0 ||
         p->dtype < NATTEN_F32 || p->dtype > NATTEN_F64)
         return NATTEN_E_INVALID;
-    if (p->dtype == NATTEN_F64 || p->dim > 256) return NATTEN_E_UNSUPPORTED;
+    if (p->dtype == NATTEN_F64 || p->dim > 256 || p->length > kAllOfThePast / 2) return NATTEN_E_UNSUPPORTED;
     Args& A = c.A;
     A = Args{};
     A.q = q; A.kc = kc; A.vc = vc;
@@ -224,8 +230,8 @@ int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void*
     A.B = p->batch; A.L = p->length; A.Hq = p->heads_q; A.Hkv = p->heads_kv; A.G = p->heads_q / p->heads_kv; A.D = p->dim;
     A.pages = p->pages; A.page_size = p->page_size; A.table_width = p->table_width;
     A.K = p->kernel == 0 ? kAllOfThePast : std::min(p->kernel, kAllOfThePast);
-    // without a window there is one class, and classes that no two tokens can be in are all alike
-    A.dil = p->kernel == 0 ? 1 : p->dilation;
+    // without a window there is one class
+    A.dil = p->kernel == 0 ? 1 : std::min(p->dilation, kAllOfThePast);
     A.by_page = FastDiv((uint32_t)p->page_size);
     A.scale_log2 = (float)(p->scale * 1.4426950408889634);
     if (A.B == 0 || A.L == 0) return NATTEN_OK;

@@ -39,11 +39,12 @@ struct Args {
     int B, L, Hq, Hkv, G, D;
     int pages, page_size, table_width;
     int K, dil;                              // window, at most kAllOfThePast
-    int M, keys, overhead, least;            // rows and keys of a tile; in key tiles: what beginning a unit costs, a CTA's least piece
-    int whole;                               // units are not shared
-    int align;                               // tiles start at multiples of it (1 with a dilation)
+    int M, keys, overhead, least;            // rows and keys (a power of two) of a tile; in key tiles: what beginning a unit costs, a CTA's least piece
+    int keys_log, whole;                     // units are not shared (whole)
+    int align;                               // tiles start at multiples of it: a power of two, 1 with a dilation
     int long_classes, tiles_long, tiles_short, per_seq, columns, ctas;
-    FastDiv by_page, by_group;
+    FastDiv by_page, by_group, by_dil, by_seq, by_long, by_short;      // by page_size, G, dil, per_seq, tiles_long, tiles_short
+    int capacity;                            // positions below it have a place in the page table
     float scale_log2;                        // scale * log2(e)
 };
 
@@ -65,38 +66,44 @@ struct Tile {                                // a row tile of a class of a seque
     int lo, hi, base, n;                     // keys lo ... hi (t), in n tiles from base on
 };
 
+// Called several times in front of a unit's first load, one call behind the other: products and shifts instead of divisions (a
+// step of one token against a window of 255 took 12.6 us with them).
 __device__ __forceinline__ Tile tile_of(const Args& A, int column)
 {
     Tile x;
-    x.b = column / A.per_seq;
-    int k = column - x.b * A.per_seq, queries = A.L / A.dil;
+    x.b = A.by_seq.div(column);
+    const int fresh = A.seq_lens ? A.seq_lens[x.b] : A.L, held = A.cache_lens[x.b];
+    int k = column - x.b * A.per_seq, queries = A.by_dil.div(A.L);
     if (k < A.long_classes * A.tiles_long) {
-        x.cls = k / A.tiles_long;
+        x.cls = A.by_long.div(k);
         k -= x.cls * A.tiles_long;
         ++queries;
     } else {
         k -= A.long_classes * A.tiles_long;
-        const int c = k / A.tiles_short;
+        const int c = A.by_short.div(k);
         x.cls = A.long_classes + c;
         k -= c * A.tiles_short;
     }
     x.row0 = k * A.M;
     x.rows = min(A.M, queries * A.G - x.row0);
-    x.fresh = A.seq_lens ? min(max(A.seq_lens[x.b], 0), A.L) : A.L;
-    const int p = min(max(A.cache_lens[x.b], 0), kAllOfThePast) - x.fresh + x.cls;      // position of the class's first query
-    x.t0 = p >= 0 ? p / A.dil : -((-p + A.dil - 1) / A.dil);
+    x.fresh = min(max(fresh, 0), A.L);
+    const int p = min(max(held, 0), kAllOfThePast) - x.fresh + x.cls;   // position of the class's first query
+    x.t0 = p >= 0 ? A.by_dil.div(p) : -A.by_dil.div(-p + A.dil - 1);
     x.residue = p - x.t0 * A.dil;
-    const int live = x.fresh > x.cls ? (x.fresh - x.cls + A.dil - 1) / A.dil : 0;
-    const int first = x.row0 / A.G, last = min((x.row0 + x.rows - 1) / A.G, live - 1);
-    const long long capacity = (long long)A.table_width * A.page_size;  // no position behind it exists
-    x.hi = x.t0 + last;
-    if (capacity <= x.residue) x.hi = -1;
-    else if (x.hi > (capacity - 1 - x.residue) / A.dil) x.hi = (int)((capacity - 1 - x.residue) / A.dil);
+    const int live = x.fresh > x.cls ? A.by_dil.div(x.fresh - x.cls + A.dil - 1) : 0;
+    const int first = A.by_group.div(x.row0), last = min(A.by_group.div(x.row0 + x.rows - 1), live - 1);
+    x.hi = A.capacity <= x.residue ? -1 : min(x.t0 + last, A.by_dil.div(A.capacity - 1 - x.residue));
     const int back = x.t0 + first - (A.K - 1);
     x.lo = x.t0 + first > 0 && back > 0 ? back : 0;
-    x.base = x.lo - x.lo % A.align;
-    x.n = last >= first && x.hi >= x.lo ? (x.hi - x.base) / A.keys + 1 : 0;
+    x.base = x.lo & ~(A.align - 1);
+    x.n = last >= first && x.hi >= x.lo ? ((x.hi - x.base) >> A.keys_log) + 1 : 0;
     return x;
+}
+
+// 64-bit division is a long subroutine, and these numbers hardly ever need it.
+__device__ __forceinline__ long long quotient(long long a, int b)
+{
+    return (unsigned long long)a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
 
 // A CTA's piece, unit by unit.  `begin` is called by all `kThreads` threads; the rest is uniform arithmetic.
@@ -133,9 +140,9 @@ struct Piece {
         }
         const long long from = before + upto - mine;
         // no CTA gets less than `least`: every piece of a unit then has tiles, and a unit's CTAs are consecutive
-        const int n = (int)min((long long)A.ctas, max(total / A.least, 1ll));
+        const int n = (int)min((long long)A.ctas, max(quotient(total, A.least), 1ll));
         pieces = n;
-        share = total / n;
+        share = quotient(total, n);
         rest = total - share * n;
         const long long start = start_of(cta), stop = start_of(cta + 1);
         if (start >= from && start < from + mine) {
@@ -156,13 +163,13 @@ struct Piece {
             column = (int)found[0];
             tile = tile_of(A, column);
             const int w = tile.n + A.overhead;
-            h = (int)(found[1] / w);
+            h = (int)quotient(found[1], w);
             off = (int)(found[1] - (long long)h * w);
             if (A.whole && off > 0) advance(A);              // another CTA's
         }
     }
     // where CTA c's piece starts: total * c / pieces, without overflow
-    __device__ __forceinline__ long long start_of(int c) const { return c < pieces ? share * c + rest * c / pieces : share * pieces + rest; }
+    __device__ __forceinline__ long long start_of(int c) const { return c < pieces ? share * c + quotient(rest * c, pieces) : share * pieces + rest; }
     // CTAs from `cta` on that share the unit that its piece ends inside of
     __device__ int parts(const Args& A, int cta) const
     {

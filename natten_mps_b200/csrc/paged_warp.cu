@@ -1,11 +1,11 @@
 // Attention over a paged cache for few rows a unit (decoding steps, a few proposed tokens), 16-bit types: warp-level matrix
 // products, each warp on its own keys.
 //
-// Such calls are bound by reading the cache: with 16 rows a key of 128 channels is 512 bytes against 4 Kflop a row.  So a CTA's
-// four warps share a unit's rows and split its keys: of a tile of 4 * NK keys a warp fetches NK of its own (asynchronous 16-byte
+// Such calls are bound by reading the cache: with 16 rows a key of 128 channels is 512 bytes against 8 Kflop.  So a CTA's
+// eight warps (four above 128 channels) share a unit's rows and split its keys: of a tile of 8 * NK keys a warp fetches NK of its own (asynchronous 16-byte
 // copies, kStages - 1 steps ahead, rows found through the page table one step before that), multiplies, runs its own softmax with
 // its own maximum, and accumulates all channels of its weighted sum in registers.  Nothing in the loop waits for another warp.
-// At the end of the unit the four partial results are joined through shared memory.
+// At the end of the unit the warps' partial results are joined through shared memory.
 //
 // A key that no row of the unit sees (behind the last query, in front of the first window, on a page that is not there) is not
 // fetched: its line of shared memory is zero.  One that some rows see and others do not is multiplied by a weight of zero in those,
@@ -32,10 +32,9 @@ using tcplan::fast_exp2;
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
-
 // MT: tiles of 16 rows; DP: head dim rounded up to 32, 64, 128 or 256
 template <int DP, int MT> struct Cfg {
+    static constexpr int kWarps = DP == 256 ? 4 : 8, kThreads = 32 * kWarps;
     static constexpr int kKeys = DP <= 64 ? 32 : 16;             // keys of a warp's step
     static constexpr int kStages = 3;
     static constexpr int kRowBytes = DP * 2, kChunks = DP / 8;   // 16-byte chunks of a row
@@ -48,7 +47,6 @@ template <int DP, int MT> struct Cfg {
     static constexpr int kStageBytes = kWarps * kWarpBytes > kExchange ? kWarps * kWarpBytes : kExchange;
     static constexpr int kSums = kQ + kStageBytes;               // float2 [kWarps][kRows], unsigned [kWarps][kStages], scratch
     static constexpr int kSmem = kSums + kWarps * kRows * 8 + kWarps * kStages * 4 + 16 + 36 * 8;
-    static constexpr int kPerSm = DP == 256 ? 1 : 2;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
@@ -66,10 +64,10 @@ template <int DP> __device__ __forceinline__ uint32_t at(int r, int c)
 }
 
 template <int DP, int MT, bool BF16>
-__global__ void __launch_bounds__(kThreads, Cfg<DP, MT>::kPerSm) warp_kernel(const __grid_constant__ Args A)
+__global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __grid_constant__ Args A)
 {
     using C = Cfg<DP, MT>;
-    constexpr int NK = C::kKeys, NT = NK / 8, ST = C::kStages;
+    constexpr int NK = C::kKeys, NT = NK / 8, ST = C::kStages, kWarps = C::kWarps, kThreads = C::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
     float2* sums = reinterpret_cast<float2*>(smem + C::kSums);
     volatile unsigned* there_words = reinterpret_cast<unsigned*>(smem + C::kSums + kWarps * C::kRows * 8);
@@ -177,11 +175,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, MT>::kPerSm) warp_kernel(con
             const unsigned seen = there_words[warp * ST + s];
             if (seen == 0u) continue;
             const uint32_t k_src = stage_base + s * 2 * C::kTile, v_src = k_src + C::kTile;
-            float sc[MT][NT][4];
+            // two sums a score (even and odd steps along the channels): half the chain of dependent products
+            float sc[MT][NT][4], odd[MT][NT][4];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) sc[m][n][0] = sc[m][n][1] = sc[m][n][2] = sc[m][n][3] = 0.f;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[m][n][e] = odd[m][n][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
@@ -190,8 +191,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, MT>::kPerSm) warp_kernel(con
                     wmma16::ldsm_x4(b, k_src + at<DP>(8 * n + (mi >> 1) * 8 + mr, 2 * k + (mi & 1)));
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
-                        wmma16::mma_16816<BF16>(sc[m][n], qf[m][k], b[0], b[1]);
-                        wmma16::mma_16816<BF16>(sc[m][n + 1], qf[m][k], b[2], b[3]);
+                        wmma16::mma_16816<BF16>(k & 1 ? odd[m][n] : sc[m][n], qf[m][k], b[0], b[1]);
+                        wmma16::mma_16816<BF16>(k & 1 ? odd[m][n + 1] : sc[m][n + 1], qf[m][k], b[2], b[3]);
                     }
                 }
             const unsigned every = NK == 32 ? 0xffffffffu : (1u << NK) - 1u;
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, MT>::kPerSm) warp_kernel(con
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float v = sc[m][n][e] * A.scale_log2;
+                        float v = (sc[m][n][e] + odd[m][n][e]) * A.scale_log2;
                         if (!open) {
                             const int j = 8 * n + 2 * (lane & 3) + (e & 1), t = base + j, to = tq[m][e >> 1];
                             if (!(((seen >> j) & 1u) && t <= to && to - t < A.K)) v = -CUDART_INF_F;
@@ -343,12 +344,12 @@ bool warp_shape(int dtype, const Args& A, bool aligned, Shape& shape)
     shape.M = rows > 16 && A.D <= 128 ? 32 : 16;
     by_config(A, shape.M, [&](auto dp, auto mt) {
         using C = Cfg<decltype(dp)::value, decltype(mt)::value>;
-        shape.keys = kWarps * C::kKeys;
-        shape.ctas = C::kPerSm * sm_count();
+        shape.keys = C::kWarps * C::kKeys;
+        shape.ctas = sm_count();
     });
     shape.overhead = 1;
     shape.least = 2;
-    shape.most = 16;
+    shape.most = 8;
     return true;
 }
 
@@ -359,7 +360,7 @@ int warp_run(int dtype, const Args& A, cudaStream_t s)
         cudaError_t err;
         auto go = [&](auto* kernel) {
             err = ensure_dynamic_smem((const void*)kernel, C::kSmem);
-            if (err == cudaSuccess) kernel<<<A.ctas, kThreads, C::kSmem, s>>>(A);
+            if (err == cudaSuccess) kernel<<<A.ctas, C::kThreads, C::kSmem, s>>>(A);
         };
         if (dtype == NATTEN_BF16) go(warp_kernel<decltype(dp)::value, decltype(mt)::value, true>);
         else go(warp_kernel<decltype(dp)::value, decltype(mt)::value, false>);
