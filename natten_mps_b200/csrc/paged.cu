@@ -196,6 +196,7 @@ bool divide(Args& A, const Shape& shape)
     A.columns = (int)(per * A.B);
     A.ctas = shape.ctas;
     A.by_group = FastDiv((uint32_t)A.G);
+    A.by_ctas = FastDiv((uint32_t)A.ctas);
     A.by_dil = FastDiv((uint32_t)A.dil);
     A.by_seq = FastDiv((uint32_t)std::max(1, A.per_seq));
     A.by_long = FastDiv((uint32_t)std::max(1, A.tiles_long));

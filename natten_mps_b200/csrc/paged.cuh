@@ -43,7 +43,7 @@ struct Args {
     int keys_log, whole;                     // units are not shared (whole)
     int align;                               // tiles start at multiples of it: a power of two, 1 with a dilation
     int long_classes, tiles_long, tiles_short, per_seq, columns, ctas;
-    FastDiv by_page, by_group, by_dil, by_seq, by_long, by_short;      // by page_size, G, dil, per_seq, tiles_long, tiles_short
+    FastDiv by_page, by_group, by_dil, by_seq, by_long, by_short, by_ctas;      // by page_size, G, dil, ...
     int capacity;                            // positions below it have a place in the page table
     float scale_log2;                        // scale * log2(e)
 };
@@ -100,82 +100,96 @@ __device__ __forceinline__ Tile tile_of(const Args& A, int column)
     return x;
 }
 
-// 64-bit division is a long subroutine, and these numbers hardly ever need it.
-__device__ __forceinline__ long long quotient(long long a, int b)
-{
-    return (unsigned long long)a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
-}
-
 // A CTA's piece, unit by unit.  `begin` is called by all `kThreads` threads; the rest is uniform arithmetic.
 struct Piece {
-    long long left, share, rest;             // the first `pieces` CTAs have `share` each, and the rest among them
-    int pieces, column, h, off;              // where the piece goes on: unit (column, h), cost `off` into it
+    long long left, total;                   // of the piece; of all pieces
+    long long share;                         // every CTA's share, and `rest` more among them; or pieces of A.least each (`few`)
+    FastDiv by_ctas;
+    int rest, pieces;
+    bool few;
+    int column, h, off;                      // where the piece goes on: unit (column, h), cost `off` into it
     Tile tile;
 
     // portion of the unit (column, h): key tiles [x0, x1).  n == 0: nothing to see, rows are to be cleared if `first`.
     struct Portion { int h, x0, x1; bool work, whole, first; };
+    // What `begin` needs of shared memory
+    struct Scratch { long long sums[32], at; int column; Tile tile; };
 
-    template <int kThreads> __device__ void begin(const Args& A, int cta, void* scratch)     // scratch: 32 + 4 long longs
+    template <int kThreads> __device__ void begin(const Args& A, int cta, Scratch* scratch)
     {
-        long long* sums = static_cast<long long*>(scratch);
-        volatile long long* found = sums + 32;
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-        const int each = (A.columns + kThreads - 1) / kThreads;
+        const int each = A.columns <= kThreads ? 1 : (A.columns + kThreads - 1) / kThreads;
         const int c0 = min(A.columns, tid * each), c1 = min(A.columns, c0 + each);
         long long mine = 0;
-        for (int c = c0; c < c1; ++c) mine += (long long)(tile_of(A, c).n + A.overhead) * A.Hkv;
+        Tile t{};
+        for (int c = c0; c < c1; ++c) {
+            t = tile_of(A, c);
+            mine += (long long)(t.n + A.overhead) * A.Hkv;
+        }
         long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long x = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += x;
         }
-        if (lane == 31) sums[warp] = upto;
+        if (lane == 31) scratch->sums[warp] = upto;
         __syncthreads();
-        long long before = 0, total = 0;
+        long long before = 0;
+        total = 0;
 #pragma unroll
         for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) before += sums[w];
-            total += sums[w];
+            if (w < warp) before += scratch->sums[w];
+            total += scratch->sums[w];
         }
         const long long from = before + upto - mine;
-        // no CTA gets less than `least`: every piece of a unit then has tiles, and a unit's CTAs are consecutive
-        const int n = (int)min((long long)A.ctas, max(quotient(total, A.least), 1ll));
-        pieces = n;
-        share = quotient(total, n);
-        rest = total - share * n;
+        // No CTA gets less than A.least: every piece of a unit then has tiles, and a unit's CTAs are consecutive.
+        few = total < (long long)A.ctas * A.least;
+        pieces = few ? max((int)total / A.least, 1) : A.ctas;
+        share = few ? A.least : total < 0x7fffffff ? A.by_ctas.div((int)total) : total / A.ctas;
+        rest = few ? 0 : (int)(total - share * A.ctas);
+        by_ctas = A.by_ctas;
         const long long start = start_of(cta), stop = start_of(cta + 1);
-        if (start >= from && start < from + mine) {
+        if (start < stop && start >= from && start < from + mine) {
             long long at = start - from;
             int c = c0;
-            for (;; ++c) {
-                const long long w = (long long)(tile_of(A, c).n + A.overhead) * A.Hkv;
-                if (at < w) break;
-                at -= w;
-            }
-            found[0] = c;
-            found[1] = at;
+            if (each > 1)
+                for (;; ++c) {
+                    t = tile_of(A, c);
+                    const long long w = (long long)(t.n + A.overhead) * A.Hkv;
+                    if (at < w) break;
+                    at -= w;
+                }
+            scratch->column = c;
+            scratch->at = at;
+            scratch->tile = t;
         }
         __syncthreads();
         left = stop - start;
         column = h = off = 0;
         if (left > 0) {
-            column = (int)found[0];
-            tile = tile_of(A, column);
-            const int w = tile.n + A.overhead;
-            h = (int)quotient(found[1], w);
-            off = (int)(found[1] - (long long)h * w);
+            column = scratch->column;
+            tile = scratch->tile;
+            const int w = tile.n + A.overhead, at = (int)scratch->at;    // less than w * Hkv
+            while (at - off >= w) {
+                off += w;
+                ++h;
+            }
+            off = at - off;
             if (A.whole && off > 0) advance(A);              // another CTA's
         }
     }
-    // where CTA c's piece starts: total * c / pieces, without overflow
-    __device__ __forceinline__ long long start_of(int c) const { return c < pieces ? share * c + quotient(rest * c, pieces) : share * pieces + rest; }
+    // where CTA c's piece starts
+    __device__ __forceinline__ long long start_of(int c) const
+    {
+        if (c >= pieces) return total;
+        return share * c + (few ? 0 : by_ctas.div(rest * c));
+    }
     // CTAs from `cta` on that share the unit that its piece ends inside of
     __device__ int parts(const Args& A, int cta) const
     {
         const long long end = start_of(cta + 1) + (tile.n + A.overhead - off - left);
         int c = cta + 1;
-        if (share > 0) c = max(c, (int)min((long long)pieces, end / (share + 1)));    // start_of(c) <= (share + 1) c
+        c = max(c, (int)min((long long)pieces, end / (share + 1)));      // start_of(c) <= (share + 1) c
         while (c < pieces && start_of(c) < end) ++c;
         return c - cta;
     }

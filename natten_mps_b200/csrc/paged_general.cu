@@ -60,7 +60,7 @@ template <typename T, int VEC, int DC>
 __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant__ Args A)
 {
     extern __shared__ __align__(16) float shared_floats[];
-    __shared__ long long scratch[36];
+    __shared__ Piece::Scratch scratch;
     __shared__ float weights[kRows][kKeys];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int padded = (A.D + 3) & ~3, pitch = padded + 4;
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant
     const T *q = static_cast<const T*>(A.q), *kc = static_cast<const T*>(A.kc), *vc = static_cast<const T*>(A.vc);
 
     Piece piece;
-    piece.begin<kThreads>(A, blockIdx.x, scratch);
+    piece.begin<kThreads>(A, blockIdx.x, &scratch);
     let_dependents_launch();
     Shared told{-1, 0};
     for (; piece.more(); piece.advance(A)) {

@@ -65,12 +65,13 @@ template <int DH, bool SPLIT> struct Cfg {
     static constexpr int kOffKV = kQ;
     static constexpr int kOffRows = kOffKV + kStages * kTile;    // long long [3][2][kKeys]: places of a tile's keys and values
     static constexpr int kOffWords = kOffRows + 3 * 2 * kKeys * 8;   // uint4 [kWordSlots]: which keys of a tile are there
-    static constexpr int kOffSums = kOffWords + kWordSlots * 16; // float2 [kHalfRows]: the second half's sums (kSplit)
+    static constexpr int kOffCopied = kOffWords + kWordSlots * 16;   // unsigned [kWordSlots]: was the tile copied row by row?
+    static constexpr int kOffSums = kOffCopied + kWordSlots * 4; // float2 [kHalfRows]: the second half's sums (kSplit)
     static constexpr int kOffBars = kOffSums + kHalfRows * 8;
     static constexpr int kBars = 2 * kStages + kWordSlots + 2 + 2 + 2 + 2 + 2 + 2;
     static constexpr int kOffFlags = kOffBars + 8 * kBars;       // abort flag, TMEM address
     static constexpr int kOffScratch = (kOffFlags + 8 + 15) & ~15;
-    static constexpr int kSmem = kOffScratch + 36 * 8;
+    static constexpr int kSmem = kOffScratch + (int)sizeof(Piece::Scratch);
     static_assert(kTile % 1024 == 0 && kSmem <= kMaxDynamicSmem, "shared memory of a CTA");
 };
 
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         tmem_alloc(smem_u32(tmem_slot), 512);
     }
     Piece piece;
-    piece.begin<kThreads>(A, blockIdx.x, smem + C::kOffScratch);
+    piece.begin<kThreads>(A, blockIdx.x, reinterpret_cast<Piece::Scratch*>(smem + C::kOffScratch));
     let_dependents_launch();
     tc_fence_before();
     __syncthreads();
@@ -187,13 +188,24 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             constexpr uint32_t idesc_qk = instr_desc(BF16 ? 1 : 0, kKeys, 0, 0), idesc_pv = instr_desc(BF16 ? 1 : 0, DH, 0, 1);
             const uint32_t leader = elect_one();
             unsigned fills = 0, units[2] = {0, 0}, tiles[2] = {0, 0};           // tiles of keys and values taken; units, tiles of each half
-            unsigned queries = 0;
+            unsigned queries = 0, seq = 0;                       // units; tiles of the CTA
+            bool copied = false;                                 // the tile whose keys came last was copied row by row
             for (; ok && piece.more(); piece.advance(A)) {
                 const Piece::Portion p = piece.portion(A);
                 if (!p.work) continue;
                 const int n = p.x1 - p.x0;
                 const bool two = SPLIT ? n > 1 : piece.tile.rows > kHalfRows;
                 auto wait_full = [&]() { ok = ok && mbar_wait(bar_full + 8 * (fills % ST), (fills / ST) & 1, abort_flag, P.wait_budget); };
+                // The keys of the next tile have landed.  Rows that threads copied are ordinary writes, which the tensor cores see
+                // behind a proxy fence (some hundred cycles on the chain of every tile: not for those that TMA brought).
+                auto wait_keys = [&]() {
+                    const unsigned w = seq % kWordSlots;
+                    ok = ok && mbar_wait(bar_words + 8 * w, (seq / kWordSlots) & 1, abort_flag, P.wait_budget);
+                    copied = reinterpret_cast<volatile unsigned*>(smem + C::kOffCopied)[w] != 0u;
+                    ++seq;
+                    wait_full();
+                    if (copied) fence_async_smem();
+                };
                 auto scores = [&](int half) {
                     const uint64_t dq = smem_desc(sbase + (SPLIT ? 0 : half * kHalfRows * 128), 16, 1024),
                                    dk = smem_desc(sbase + C::kOffKV + (fills % ST) * C::kTile, 16, 1024);
@@ -220,10 +232,10 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 };
                 ok = ok && mbar_wait(bar_q, queries & 1, abort_flag, P.wait_budget);
                 ++queries;
-                wait_full();
+                wait_keys();
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                fence_async_smem();
+                fence_async_smem();                              // the queries were copied
                 tc_fence_after();
                 if constexpr (SPLIT) {
                     // tile j belongs to half j & 1; order of the loads: K0, K1, V0, K2, V1, ...
@@ -231,17 +243,17 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     if (n == 1) mma_commit_e(bar_qfree, leader);
                     release();
                     for (int j = 0; j < n; ++j) {
+                        const bool v_copied = copied;            // tile j's; wait_keys has the next one's
                         if (j + 1 < n) {
-                            wait_full();
+                            wait_keys();
                             if (!ok) break;
-                            fence_async_smem();
                             tc_fence_after();
                             scores((j + 1) & 1);                 // after P V of tile j - 1 in issue order: over its P
                             if (j + 2 == n) mma_commit_e(bar_qfree, leader);
                             release();
                         }
                         wait_full();
-                        fence_async_smem();
+                        if (v_copied) fence_async_smem();
                         wait_p(j & 1, j < 2);
                         if (!ok) break;
                         tc_fence_after();
@@ -260,16 +272,15 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         auto next_scores = [&](int half) {
                             if (j + 1 == n) return;
                             fills = v + 1;
-                            if (half == 0) wait_full();
+                            if (half == 0) wait_keys();
                             if (ok) {
-                                if (half == 0) fence_async_smem();
                                 tc_fence_after();
                                 scores(half);
                             }
                             fills = v;
                         };
                         wait_full();
-                        fence_async_smem();
+                        if (copied) fence_async_smem();          // (still tile j's)
                         wait_p(0, j == 0);
                         if (!ok) break;
                         tc_fence_after();
@@ -351,12 +362,13 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 auto keys_of = [&](int j) {
                     Keys k{page, slot, false, places + (j % 3) * 2 * kKeys};
                     const unsigned seen = __ballot_sync(0xffffffffu, there), w = seq % kWordSlots;
+                    if (A.align > 1) k.whole = loaders_agree(there);
                     if (lane == 0) {
                         reinterpret_cast<unsigned*>(smem + C::kOffWords)[4 * w + (warp & 3)] = seen;
+                        if (warp == 8) reinterpret_cast<unsigned*>(smem + C::kOffCopied)[w] = !k.whole;
                         mbar_arrive(bar_words + 8 * w);
                     }
                     ++seq;
-                    if (A.align > 1) k.whole = loaders_agree(there);
                     if (!k.whole) {
                         long long* at = places + (j % 3) * 2 * kKeys;
                         at[lt] = there ? page * A.ks[0] + slot * A.ks[1] + p.h * A.ks[2] : -1;

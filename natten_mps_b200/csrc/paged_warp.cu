@@ -46,7 +46,7 @@ template <int DP, int MT> struct Cfg {
     static constexpr int kExchange = kWarps * kRows * kPitch * 4;
     static constexpr int kStageBytes = kWarps * kWarpBytes > kExchange ? kWarps * kWarpBytes : kExchange;
     static constexpr int kSums = kQ + kStageBytes;               // float2 [kWarps][kRows], unsigned [kWarps][kStages], scratch
-    static constexpr int kSmem = kSums + kWarps * kRows * 8 + kWarps * kStages * 4 + 16 + 36 * 8;
+    static constexpr int kSmem = kSums + kWarps * kRows * 8 + kWarps * kStages * 4 + 16 + (int)sizeof(Piece::Scratch);
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
     extern __shared__ __align__(128) unsigned char smem[];
     float2* sums = reinterpret_cast<float2*>(smem + C::kSums);
     volatile unsigned* there_words = reinterpret_cast<unsigned*>(smem + C::kSums + kWarps * C::kRows * 8);
-    long long* scratch = reinterpret_cast<long long*>(smem + C::kSums + kWarps * C::kRows * 8 + ((kWarps * ST * 4 + 15) & ~15));
+    Piece::Scratch* scratch = reinterpret_cast<Piece::Scratch*>(smem + C::kSums + kWarps * C::kRows * 8 + ((kWarps * ST * 4 + 15) & ~15));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t q_base = smem_u32(smem), stage_base = q_base + C::kQ + warp * C::kWarpBytes;
     const uint16_t *q = static_cast<const uint16_t*>(A.q), *kc = static_cast<const uint16_t*>(A.kc), *vc = static_cast<const uint16_t*>(A.vc);
@@ -89,13 +89,15 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
 
         const int steps = p.x1 - p.x0, first_key = x.lo + p.x0 * (kWarps * NK) + warp * NK;
         // ---- fetching ----
-        int page = 0, slot = 0;
-        bool there = false;
+        struct Place { int page, slot; bool there; };
         auto look_up = [&](int step) {       // lane's key of the step: its place in the cache
-            const int t = first_key + step * (kWarps * NK) + lane;
-            there = step < steps && lane < NK && locate(A, x, t, page, slot);
+            Place y{0, 0, false};
+            y.there = step < steps && lane < NK && locate(A, x, first_key + step * (kWarps * NK) + lane, y.page, y.slot);
+            return y;
         };
-        auto fetch = [&](int step) {         // uses what look_up(step) found
+        auto fetch = [&](int step, const Place& y) {
+            const int page = y.page, slot = y.slot;
+            const bool there = y.there;
             if (step < steps) {
                 const unsigned seen = __ballot_sync(0xffffffffu, there);
                 const int s = step % ST;
@@ -119,7 +121,9 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
         };
 
         // ---- the unit's queries ----
-        look_up(0);
+        Place ahead[ST];                     // of the first steps, all asked for at once; then ahead[0]: of the next step to fetch
+#pragma unroll
+        for (int s = 0; s < ST; ++s) ahead[s] = look_up(s);
         for (int e = tid; e < C::kRows * C::kChunks; e += kThreads) {
             const int r = e / C::kChunks, c = e % C::kChunks;
             const bool here = r < x.rows && c * 8 < A.D;
@@ -127,10 +131,8 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
         }
         copies_commit();
 #pragma unroll
-        for (int s = 0; s < ST - 1; ++s) {
-            fetch(s);
-            look_up(s + 1);
-        }
+        for (int s = 0; s < ST - 1; ++s) fetch(s, ahead[s]);
+        ahead[0] = ahead[ST - 1];
         int tq[MT][2], t_least = 0x7fffffff, t_most = -1;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -169,8 +171,8 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
         for (int step = 0; step < steps; ++step) {
             copies_wait<ST - 2>();
             __syncwarp();                    // every lane's copies of this step have landed, and the last step's buffers have been read
-            fetch(step + ST - 1);
-            look_up(step + ST);
+            fetch(step + ST - 1, ahead[0]);
+            ahead[0] = look_up(step + ST);
             const int s = step % ST, base = first_key + step * (kWarps * NK);
             const unsigned seen = there_words[warp * ST + s];
             if (seen == 0u) continue;
@@ -275,9 +277,9 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
         const bool direct = clear || p.whole;
         const int where = 2 * (int)blockIdx.x + (p.x0 == 0 ? 1 : 0);
         if (!direct && p.x0 == 0) told = {piece.column * A.Hkv + p.h, piece.parts(A, blockIdx.x)};
-        const int chunks = A.D / 8;
-        for (int e = tid; e < x.rows * chunks; e += kThreads) {
-            const int r = e / chunks, c = e - r * chunks;
+        for (int e = tid; e < x.rows * C::kChunks; e += kThreads) {
+            const int r = e / C::kChunks, c = e % C::kChunks;
+            if (8 * c >= A.D) continue;
             float m = -CUDART_INF_F, l = 0.f, f[kWarps], o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) m = fmaxf(m, sums[k * C::kRows + r].x);
