@@ -103,14 +103,18 @@ __device__ __forceinline__ void exp2_fma(uint64_t e, float& a, float& b)
     a = __uint_as_float(__float_as_uint(lo_of(y)) + (__float_as_uint(lo_of(r)) << 23));
     b = __uint_as_float(__float_as_uint(hi_of(y)) + (__float_as_uint(hi_of(r)) << 23));
 }
-// The loads of this thread's TMEM rows have landed: nothing that uses them may move in front of this.
-__device__ __forceinline__ void landed(uint32_t (&r)[32])
+// The loads of this thread's TMEM rows have landed.  What is done with them takes the returned factor, so that none of it can move
+// in front of the wait.  (The loaded registers as operands of the wait would say the same, but cost two moves each: 250 of a
+// tile's 900 instructions.)
+__device__ __forceinline__ uint64_t landed(uint64_t factor)
 {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
-                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
-                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+l"(factor) :: "memory");
+    return factor;
+}
+__device__ __forceinline__ float landed(float factor)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(factor) :: "memory");
+    return factor;
 }
 // barrier 1 of the 128 loading threads; true if every one of them brought true
 __device__ __forceinline__ bool loaders_agree(bool ok)
@@ -268,37 +272,30 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     if (n == 1) mma_commit_e(bar_qfree, leader);
                     release();
                     for (int j = 0; j < n; ++j) {
+                        // Everything that can be waited for ahead is: what lies between a half's P and its next S is on the chain
+                        // of every tile.
                         const unsigned v = fills;                // V of the tile; K of the next one follows it
-                        auto next_scores = [&](int half) {
-                            if (j + 1 == n) return;
-                            fills = v + 1;
-                            if (half == 0) wait_keys();
-                            if (ok) {
-                                tc_fence_after();
-                                scores(half);
-                            }
-                            fills = v;
-                        };
+                        const bool more = j + 1 < n;
                         wait_full();
                         if (copied) fence_async_smem();          // (still tile j's)
-                        wait_p(0, j == 0);
-                        if (!ok) break;
-                        tc_fence_after();
-                        weighted(0, j == 0);
-                        if (j + 1 == n) mma_commit_e(bar_o, leader);
-                        next_scores(0);
-                        if (two) {
-                            wait_p(1, j == 0);
-                            if (!ok) break;
+                        fills = v + 1;
+                        if (more) wait_keys();
+                        auto half_of = [&](int half) {
+                            wait_p(half, j == 0);
+                            if (!ok) return;
                             tc_fence_after();
-                            weighted(1, j == 0);
-                            if (j + 1 == n) mma_commit_e(bar_o + 8, leader);
-                        }
-                        release();                               // V
-                        if (j + 1 < n) {
                             fills = v;
-                            if (two) next_scores(1);
+                            weighted(half, j == 0);
+                            if (!more) mma_commit_e(bar_o + 8 * half, leader);
                             fills = v + 1;
+                            if (more) scores(half);
+                        };
+                        half_of(0);
+                        if (two && ok) half_of(1);
+                        if (!ok) break;
+                        fills = v;
+                        release();                               // V
+                        if (more) {
                             if (j + 2 == n) mma_commit_e(bar_qfree, leader);
                             release();                           // K of the next tile
                         }
@@ -462,9 +459,9 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     for (int part = 0; part < DH / 16; ++part) {
                         uint32_t o[16];
                         tmem_ld16(ocol + 16 * part, o);
-                        tmem_ld_wait();
+                        const float by = landed(f);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
                         tmem_st16(ocol + 16 * part, o);
                     }
                 }
@@ -472,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 for (int pc = 0; pc < pieces; ++pc) {
                     uint32_t w[16];
                     tmem_ld16(scol + 16 * pc, w);
-                    tmem_ld_wait();
+                    const float by = landed(f);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float a, b;
@@ -484,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             a = __low2float(h2);
                             b = __high2float(h2);
                         }
-                        w[i] = cvt_pack<BF16>(a * f, b * f);
+                        w[i] = cvt_pack<BF16>(a * by, b * by);
                     }
                     tmem_st16(scol + 16 * pc, w);
                 }
@@ -509,19 +506,19 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 bool stored = false;
                 if ((words[0] & words[1] & words[2] & words[3]) == 0xffffffffu && base + kKeys - 1 <= t_least && t_most - base < A.K &&
                     !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
-                    uint32_t s[2][32], pk[4][16];
+                    uint32_t s[4][32], pk[4][16];                // all columns at once: one wait, and nothing drains in between
                     const uint64_t nb2 = pack2(-m, -m);
                     uint64_t sum0 = 0ull, sum1 = 0ull;
-                    tmem_ld32(scol, s[0]);
-                    landed(s[0]);
+#pragma unroll
+                    for (int pc = 0; pc < 4; ++pc) tmem_ld32(scol + 32 * pc, s[pc]);
+                    const uint64_t by2 = landed(sc2);
 #pragma unroll
                     for (int pc = 0; pc < 4; ++pc) {
-                        if (pc < 3) tmem_ld32(scol + 32 * (pc + 1), s[(pc + 1) & 1]);
-                        uint32_t(&x)[32] = s[pc & 1];
+                        uint32_t(&x)[32] = s[pc];
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            const uint64_t e = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, nb2);
-                            const uint64_t g = fma2(pack2(__uint_as_float(x[2 * i + 2]), __uint_as_float(x[2 * i + 3])), sc2, nb2);
+                            const uint64_t e = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), by2, nb2);
+                            const uint64_t g = fma2(pack2(__uint_as_float(x[2 * i + 2]), __uint_as_float(x[2 * i + 3])), by2, nb2);
                             float a = 0.f, b = 0.f;
                             if (i % 6 == 0) exp2_fma(e, a, b);
                             else {
@@ -534,7 +531,6 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             pk[pc][i] = cvt_pack<BF16>(a, b);
                             pk[pc][i + 1] = cvt_pack<BF16>(c, d);
                         }
-                        if (pc < 3) landed(s[(pc + 1) & 1]);
                     }
                     sum0 = add2(sum0, sum1);
                     const float rs = lo_of(sum0) + hi_of(sum0);
@@ -558,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     }
                     uint32_t s[32];
                     tmem_ld32(scol + 32 * pc, s);
-                    landed(s);
+                    const uint64_t by2 = landed(sc2);
+                    const float by = lo_of(by2);
                     // every row of the warp that counts sees all of the piece
                     const bool open = word == 0xffffffffu && t0 + 31 <= t_least && t_most - t0 < A.K;
                     uint32_t bits = 0xffffffffu;
@@ -567,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         float top = -CUDART_INF_F;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * A.scale_log2);
+                            if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * by);
                         if (m == -CUDART_INF_F) m = top;
                     }
                     bool done = false;
@@ -577,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         float sum_a = 0.f, sum_b = 0.f;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const uint64_t e = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, nb2);
+                            const uint64_t e = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), by2, nb2);
                             float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e));
                             if (!open) {                         // whatever a hidden score gave
                                 a = (bits >> (2 * i)) & 1u ? a : 0.f;
@@ -598,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         float over = -CUDART_INF_F;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const float e = (bits >> i) & 1u ? fmaf(__uint_as_float(s[i]), A.scale_log2, -base_m) : -CUDART_INF_F;
+                            const float e = (bits >> i) & 1u ? fmaf(__uint_as_float(s[i]), by, -base_m) : -CUDART_INF_F;
                             s[i] = __float_as_uint(e);
                             over = fmaxf(over, e);
                         }
@@ -659,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 tc_fence_after();
             }
             const bool some = live && l != 0.f;                  // (a NaN stays one)
-            const float inv = direct ? (some ? 1.f / l : 0.f) : 1.f;
+            float inv = direct ? (some ? 1.f / l : 0.f) : 1.f;
             const bool both = SPLIT && n > 1;
             // Four lanes exchange 16-byte pieces, so that a store writes 64 bytes of each of eight rows.
             long long rows4[4];
@@ -672,18 +669,19 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 uint32_t o[32];
                 if (n > 0) {
                     tmem_ld32(ocol + 32 * part, o);
-                    landed(o);
                     if (both) {
+                        uint32_t y[32];
+                        tmem_ld32(trow + kColO + 128 + 32 * part, y);
+                        const uint64_t mine2 = landed(pack2(f_mine, f_mine)), other2 = pack2(f_other, f_other);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t y[16];
-                            tmem_ld16(trow + kColO + 128 + 32 * part + 16 * h, y);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                o[16 * h + i] = __float_as_uint(__uint_as_float(o[16 * h + i]) * f_mine + __uint_as_float(y[i]) * f_other);
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t z = fma2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), mine2,
+                                                    tcplan::mul2(pack2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), other2));
+                            o[2 * i] = __float_as_uint(lo_of(z));
+                            o[2 * i + 1] = __float_as_uint(hi_of(z));
                         }
                     }
+                    inv = landed(inv);
                 }
                 if (direct) {
                     uint32_t y[4][4];
@@ -705,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) y[i][k] = o[16 * h + 4 * i + k];
+                            for (int k = 0; k < 4; ++k) y[i][k] = __float_as_uint(__uint_as_float(o[16 * h + 4 * i + k]) * inv);    // (times 1)
                         transpose4(y, piece4);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
