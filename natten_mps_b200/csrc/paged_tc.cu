@@ -16,10 +16,10 @@
 //
 // Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products.  The loading threads look the keys
 // of a tile up in the page table, a tile ahead.  Where 16 or more keys at a time are adjacent in a page (no dilation, a page
-// size that is a multiple of 16) tiles start at such a run and TMA brings one run of a tile that is there as a whole.  The other
-// tiles (the first and last of a unit, pages of other sizes, dilated keys) are copied row by row, 16 bytes at a time, into the
-// same swizzled layout; a row that is not there is zero, whatever its slot holds.  Row-wise copies of every tile would take 3750
-// cycles a tile, twice what the products need.
+// size that is a multiple of 16) tiles start at such a run, and TMA brings the runs that are there as a whole.  The other keys
+// (of runs that a unit's first and last key cut, pages of other sizes, dilated keys) are copied row by row, 16 bytes at a time,
+// into the same swizzled layout; a row that is not there is zero, whatever its slot holds.  Row-wise copies of every tile would
+// take 3750 cycles a tile, twice what the products need.  The queries come by TMA where a group's heads divide the tile, too.
 //
 // TMEM columns: S (P over its first half) of the halves at 0 and 128, O at 256 and 384.
 #include "../../include/natten_b200.h"
@@ -54,7 +54,7 @@ constexpr int kThreads = 512, kKeys = 128, kHalfRows = 128, kWordSlots = 16;
 constexpr int kSoftmaxRegs = 176, kHelperRegs = 80;              // 2 x 128 x (176 + 80) = the 65536 of the launch
 constexpr uint32_t kColO = 256;
 
-struct Status { int* status; int* status_host; long long wait_budget; int inject; };
+struct Status { int* status; int* status_host; long long wait_budget; int inject, boxed; };      // boxed: queries come by TMA
 
 template <int DH, bool SPLIT> struct Cfg {
     static constexpr int kBlocks = DH / 64;                      // 64-channel blocks: rows of 128 bytes, 128-byte swizzle
@@ -65,7 +65,7 @@ template <int DH, bool SPLIT> struct Cfg {
     static constexpr int kOffKV = kQ;
     static constexpr int kOffRows = kOffKV + kStages * kTile;    // long long [3][2][kKeys]: places of a tile's keys and values
     static constexpr int kOffWords = kOffRows + 3 * 2 * kKeys * 8;   // uint4 [kWordSlots]: which keys of a tile are there
-    static constexpr int kOffCopied = kOffWords + kWordSlots * 16;   // unsigned [kWordSlots]: was the tile copied row by row?
+    static constexpr int kOffCopied = kOffWords + kWordSlots * 16;   // unsigned [kWordSlots]: were rows of the tile copied?
     static constexpr int kOffSums = kOffCopied + kWordSlots * 4; // float2 [kHalfRows]: the second half's sums (kSplit)
     static constexpr int kOffBars = kOffSums + kHalfRows * 8;
     static constexpr int kBars = 2 * kStages + kWordSlots + 2 + 2 + 2 + 2 + 2 + 2;
@@ -103,6 +103,11 @@ __device__ __forceinline__ void exp2_fma(uint64_t e, float& a, float& b)
     a = __uint_as_float(__float_as_uint(lo_of(y)) + (__float_as_uint(lo_of(r)) << 23));
     b = __uint_as_float(__float_as_uint(hi_of(y)) + (__float_as_uint(hi_of(r)) << 23));
 }
+// The barrier's phase waits for these bytes, too (no arrival).
+__device__ __forceinline__ void mbar_expect_bytes(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 // The loads of this thread's TMEM rows have landed.  What is done with them takes the returned factor, so that none of it can move
 // in front of the wait.  (The loaded registers as operands of the wait would say the same, but cost two moves each: 250 of a
 // tile's 900 instructions.)
@@ -126,7 +131,8 @@ __device__ __forceinline__ bool loaders_agree(bool ok)
 }
 
 template <int DH, bool BF16, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Args A,
+__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+          const __grid_constant__ Args A,
           const __grid_constant__ Status P)
 {
     using C = Cfg<DH, SPLIT>;
@@ -193,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             const uint32_t leader = elect_one();
             unsigned fills = 0, units[2] = {0, 0}, tiles[2] = {0, 0};           // tiles of keys and values taken; units, tiles of each half
             unsigned queries = 0, seq = 0;                       // units; tiles of the CTA
-            bool copied = false;                                 // the tile whose keys came last was copied row by row
+            bool copied = false;                                 // rows of the tile whose keys came last were copied
             for (; ok && piece.more(); piece.advance(A)) {
                 const Piece::Portion p = piece.portion(A);
                 if (!p.work) continue;
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 wait_keys();
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                fence_async_smem();                              // the queries were copied
+                if (!P.boxed) fence_async_smem();
                 tc_fence_after();
                 if constexpr (SPLIT) {
                     // tile j belongs to half j & 1; order of the loads: K0, K1, V0, K2, V1, ...
@@ -319,8 +325,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             unsigned fills = 0, seq = 0, queries = 0;
             auto wait_empty = [&](uint32_t b, uint32_t parity) { ok = ok && mbar_wait(b, parity, abort_flag, P.wait_budget); };
             // A tile's keys: this thread's (the lt-th) page and slot, and where the keys and values of all of them are (elements).
-            // whole: every key is there, and they come in runs of A.align.
-            struct Keys { int page, slot; bool whole; const long long* at; };
+            // runs: bit i is set where the run of A.align keys that key i * 16 belongs to is there as a whole.
+            struct Keys { int page, slot; unsigned runs; const long long* at; };
             for (; ok && piece.more(); piece.advance(A)) {
                 const Piece::Portion p = piece.portion(A);
                 if (!p.work) continue;
@@ -330,20 +336,25 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     const unsigned s = fills % ST;
                     const uint32_t full = bar_full + 8 * s, dst = sbase + C::kOffKV + s * C::kTile;
                     if (fills >= (unsigned)ST) wait_empty(bar_empty + 8 * s, (fills / ST - 1) & 1);
-                    if (ok && k.whole) {
-                        if (lt == 0) mbar_expect_tx(full, C::kTile);
-                        else mbar_arrive(full);
-                        if ((lt & (A.align - 1)) == 0)
+                    if (ok) {
+                        if (lt == 0 && k.runs) mbar_expect_bytes(full, __popc(k.runs) * (C::kTile / 8));
+                        if (((k.runs >> (lt >> 4)) & 1u) && (lt & (A.align - 1)) == 0)
 #pragma unroll
                             for (int b = 0; b < C::kBlocks; ++b)
                                 tma_load_5d(dst + b * C::kBlock + lt * 128, map, full, 0, k.slot, b, p.h, k.page);
-                    } else if (ok) {
-#pragma unroll 4
-                        for (int r = r0; r < kKeys; r += kAtOnce) {
-                            const long long o = k.at[offset + r];
-                            copy16(dst + c_off + r * 128 + (((c ^ r) & 7) << 4), o >= 0 ? src + o + c * 8 : q, o >= 0);
+                        if (k.runs == 0xffu) {
+                            mbar_arrive(full);
+                        } else {
+                            for (int r16 = 0; r16 < kKeys; r16 += 16) {
+                                if ((k.runs >> (r16 >> 4)) & 1u) continue;
+#pragma unroll
+                                for (int r = r16 + r0; r < r16 + 16; r += kAtOnce) {
+                                    const long long o = k.at[offset + r];
+                                    copy16(dst + c_off + r * 128 + (((c ^ r) & 7) << 4), o >= 0 ? src + o + c * 8 : q, o >= 0);
+                                }
+                            }
+                            arrive_when_landed(full);
                         }
-                        arrive_when_landed(full);
                     }
                     ++fills;
                 };
@@ -357,33 +368,50 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 // Tile j (the lookup for the next one is under way while this one is copied).  Three buffers: with kSplit a thread
                 // may still copy the values of tile j - 2 when another writes the places of tile j.
                 auto keys_of = [&](int j) {
-                    Keys k{page, slot, false, places + (j % 3) * 2 * kKeys};
+                    long long* at = places + (j % 3) * 2 * kKeys;
                     const unsigned seen = __ballot_sync(0xffffffffu, there), w = seq % kWordSlots;
-                    if (A.align > 1) k.whole = loaders_agree(there);
+                    volatile unsigned* words = reinterpret_cast<volatile unsigned*>(smem + C::kOffWords) + 4 * w;
+                    if (lane == 0) words[warp & 3] = seen;
+                    at[lt] = there ? page * A.ks[0] + slot * A.ks[1] + p.h * A.ks[2] : -1;
+                    at[kKeys + lt] = there ? page * A.vs[0] + slot * A.vs[1] + p.h * A.vs[2] : -1;
+                    Keys k{page, slot, 0u, at};
+                    look_up(j + 1);
+                    ok = loaders_agree(ok);
+                    if (A.align > 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const unsigned word = words[i];
+                            unsigned whole = ((word & 0xffffu) == 0xffffu ? 1u : 0u) | (word >> 16 == 0xffffu ? 2u : 0u);
+                            if (A.align > 16) whole = whole == 3u ? 3u : 0u;
+                            k.runs |= whole << (2 * i);
+                        }
+                        if (A.align > 32) k.runs = ((k.runs & 0xfu) == 0xfu ? 0xfu : 0u) | ((k.runs & 0xf0u) == 0xf0u ? 0xf0u : 0u);
+                    }
                     if (lane == 0) {
-                        reinterpret_cast<unsigned*>(smem + C::kOffWords)[4 * w + (warp & 3)] = seen;
-                        if (warp == 8) reinterpret_cast<unsigned*>(smem + C::kOffCopied)[w] = !k.whole;
+                        if (warp == 8) reinterpret_cast<unsigned*>(smem + C::kOffCopied)[w] = k.runs != 0xffu;
                         mbar_arrive(bar_words + 8 * w);
                     }
                     ++seq;
-                    if (!k.whole) {
-                        long long* at = places + (j % 3) * 2 * kKeys;
-                        at[lt] = there ? page * A.ks[0] + slot * A.ks[1] + p.h * A.ks[2] : -1;
-                        at[kKeys + lt] = there ? page * A.vs[0] + slot * A.vs[1] + p.h * A.vs[2] : -1;
-                    }
-                    look_up(j + 1);
-                    ok = loaders_agree(ok);
                     return k;
                 };
                 auto load_queries = [&]() {
                     if (queries > 0) wait_empty(bar_qfree, (queries - 1) & 1);
-                    if (ok) {
+                    const bool tell = P.inject != 1 || queries > 0 || lt > 0;        // test hook: a barrier that never fills
+                    if (ok && P.boxed) {
+                        if (lt == 0) {
+                            mbar_expect_bytes(bar_q, C::kQ);
+#pragma unroll
+                            for (int b = 0; b < C::kBlocks; ++b)
+                                tma_load_5d(sbase + b * C::kQBlock, &tmQ, bar_q, 0, p.h * A.G, A.by_group.div(x.row0), b, x.b);
+                        }
+                        if (tell) mbar_arrive(bar_q);
+                    } else if (ok) {
 #pragma unroll 2
                         for (int r = r0; r < C::kRows; r += kAtOnce) {
                             const bool here = r < x.rows;
                             copy16(sbase + cq_off + r * 128 + (((c ^ r) & 7) << 4), here ? q + query_offset(A, x, p.h, r) + c * 8 : q, here);
                         }
-                        if (P.inject != 1 || queries > 0 || lt > 0) arrive_when_landed(bar_q);     // test hook: a barrier that never fills
+                        if (tell) arrive_when_landed(bar_q);
                     }
                     ++queries;
                 };
@@ -748,6 +776,15 @@ static bool encode_cache(CUtensorMap* map, const Args& A, bool bf16, const void*
     return tcplan::encode_16bit(map, cache, bf16, dims, bytes, box, steps);
 }
 
+// Queries, 64 channels: [64, head, token, block of 64 channels, sequence]; a box is the rows of a tile, the heads of a group first.
+static bool encode_queries(CUtensorMap* map, const Args& A, bool bf16)
+{
+    const cuuint64_t dims[5] = {64, (cuuint64_t)A.Hq, (cuuint64_t)A.L, (cuuint64_t)A.D / 64, (cuuint64_t)A.B};
+    const cuuint64_t bytes[4] = {(cuuint64_t)A.qs[2] * 2, (cuuint64_t)A.qs[1] * 2, 128, (cuuint64_t)A.qs[0] * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)A.G, (cuuint32_t)(A.M / A.G), 1, 1}, steps[5] = {1, 1, 1, 1, 1};
+    return tcplan::encode_16bit(map, A.q, bf16, dims, bytes, box, steps);
+}
+
 bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape)
 {
     if ((dtype != NATTEN_F16 && dtype != NATTEN_BF16) || !aligned || (A.D != 64 && A.D != 128)) return false;
@@ -767,17 +804,18 @@ int tc_run(int dtype, const Args& call, cudaStream_t s)
     if (err == cudaSuccess) err = tcplan::status_host_ptr(st.status_host);
     if (err != cudaSuccess) return (int)err;
     // Runs of 64, 32 or 16 adjacent keys where the page size is a multiple of that many and nothing is dilated.
-    CUtensorMap mk{}, mv{};
+    CUtensorMap mq{}, mk{}, mv{};
     if (A.dil == 1 && A.pages > 0 && A.page_size % 16 == 0) {
         const int run = A.page_size % 64 == 0 ? 64 : A.page_size % 32 == 0 ? 32 : 16;
         if (encode_cache(&mk, A, dtype == NATTEN_BF16, A.kc, A.ks, run) && encode_cache(&mv, A, dtype == NATTEN_BF16, A.vc, A.vs, run)) A.align = run;
     }
+    st.boxed = A.dil == 1 && A.M % A.G == 0 && encode_queries(&mq, A, dtype == NATTEN_BF16);
     auto go = [&](auto dh, auto bf, auto split) {
         constexpr int kDim = decltype(dh)::value;
         using C = Cfg<kDim, decltype(split)::value>;
         auto* kernel = tc_kernel<kDim, decltype(bf)::value, decltype(split)::value>;
         err = ensure_dynamic_smem((const void*)kernel, C::kSmem);
-        if (err == cudaSuccess) kernel<<<A.ctas, kThreads, C::kSmem, s>>>(mk, mv, A, st);
+        if (err == cudaSuccess) kernel<<<A.ctas, kThreads, C::kSmem, s>>>(mq, mk, mv, A, st);
     };
     auto by_rows = [&](auto dh, auto bf) {
         if (A.M == kHalfRows) go(dh, bf, std::true_type{});
