@@ -14,7 +14,9 @@
 // which the row sum of a piece tells; O, the sum and the tile's probabilities so far are then rescaled by the thread itself.  So
 // there is no running maximum, and no thread has to touch O in between.
 //
-// Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products.  The loading threads look the keys
+// Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products, one that walks the CTA's units and
+// hands them to the others (what a unit is takes some hundred instructions and the sequence's lengths, which would stand in
+// front of every unit in every role; and the less code the roles have, the less of it is fetched again for every unit).  The loading threads look the keys
 // of a tile up in the page table, a tile ahead.  Where 16 or more keys at a time are adjacent in a page (no dilation, a page
 // size that is a multiple of 16) tiles start at such a run, and TMA brings the runs that are there as a whole.  The other keys
 // (of runs that a unit's first and last key cut, pages of other sizes, dilated keys) are copied row by row, 16 bytes at a time,
@@ -50,9 +52,16 @@ using tcplan::transpose4;
 
 namespace {
 
-constexpr int kThreads = 512, kKeys = 128, kHalfRows = 128, kWordSlots = 16;
+constexpr int kThreads = 512, kKeys = 128, kHalfRows = 128, kWordSlots = 16, kUnitSlots = 4;
 constexpr int kSoftmaxRegs = 176, kHelperRegs = 80;              // 2 x 128 x (176 + 80) = the 65536 of the launch
 constexpr uint32_t kColO = 256;
+
+// A unit, or a CTA's part of one: key tiles [x0, x1) of a row tile and a key/value head.
+enum : int { kEnd, kWork, kClear };          // kClear: no row sees anything
+struct Unit {
+    int kind, h, x0, x1, direct;             // direct: rows are written out; else to the CTA's slot of partial results
+    Tile tile;
+};
 
 struct Status { int* status; int* status_host; long long wait_budget; int inject, boxed; };      // boxed: queries come by TMA
 
@@ -68,10 +77,11 @@ template <int DH, bool SPLIT> struct Cfg {
     static constexpr int kOffCopied = kOffWords + kWordSlots * 16;   // unsigned [kWordSlots]: were rows of the tile copied?
     static constexpr int kOffSums = kOffCopied + kWordSlots * 4; // float2 [kHalfRows]: the second half's sums (kSplit)
     static constexpr int kOffBars = kOffSums + kHalfRows * 8;
-    static constexpr int kBars = 2 * kStages + kWordSlots + 2 + 2 + 2 + 2 + 2 + 2;
+    static constexpr int kBars = 2 * kStages + kWordSlots + 2 + 2 + 2 + 2 + 2 + 2 + 2 * kUnitSlots;
     static constexpr int kOffFlags = kOffBars + 8 * kBars;       // abort flag, TMEM address
     static constexpr int kOffScratch = (kOffFlags + 8 + 15) & ~15;
-    static constexpr int kSmem = kOffScratch + (int)sizeof(Piece::Scratch);
+    static constexpr int kOffUnits = (kOffScratch + (int)sizeof(Piece::Scratch) + 15) & ~15;      // Unit [kUnitSlots]
+    static constexpr int kSmem = kOffUnits + kUnitSlots * (int)sizeof(Unit);
     static_assert(kTile % 1024 == 0 && kSmem <= kMaxDynamicSmem, "shared memory of a CTA");
 };
 
@@ -155,6 +165,9 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     const uint32_t bar_ofree = bar_o + 16;                       // [2] O has been read
     const uint32_t bar_sums = bar_ofree + 16;                    // [2] kSplit: the second half's sums are in shared memory; have been read
 
+    const uint32_t bar_unit = bar_sums + 16;                     // [kUnitSlots] the unit is there
+    const uint32_t bar_unitfree = bar_unit + 8 * kUnitSlots;     // [kUnitSlots] ... has been read by the 13 warps that use it
+
     if (warp == 12) {
         if (lane == 0) {
             // swizzled tiles need a 1024-byte aligned base; once any CTA has given up, the rest bail out
@@ -164,6 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 mbar_init(bar_empty + 8 * i, 1);
             }
             for (int i = 0; i < kWordSlots; ++i) mbar_init(bar_words + 8 * i, 4);
+            for (int i = 0; i < kUnitSlots; ++i) {
+                mbar_init(bar_unit + 8 * i, 1);
+                mbar_init(bar_unitfree + 8 * i, 13);
+            }
             mbar_init(bar_q, 128);
             mbar_init(bar_qfree, 1);
             for (int i = 0; i < 2; ++i) {
@@ -186,11 +203,58 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    Shared told{-1, 0};
+    const Unit* units_at = reinterpret_cast<const Unit*>(smem + C::kOffUnits);
+    // The CTA's next unit (kEnd after the last one, or when some wait ran out), for a warp.
+    auto next_unit = [&](unsigned& walked) {
+        const unsigned slot = walked % kUnitSlots;
+        Unit u;
+        u.kind = kEnd;
+        if (warp_wait(bar_unit + 8 * slot, (walked / kUnitSlots) & 1, abort_flag, P.wait_budget)) {
+            u = units_at[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_unitfree + 8 * slot);
+        }
+        ++walked;
+        return u;
+    };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
-        if (warp == 12) {
+        if (warp == 13) {
+            // =====================================================================
+            // Units
+            // =====================================================================
+            Shared told{-1, 0};
+            for (unsigned walked = 0; !gave_up(abort_flag); ++walked) {
+                Piece::Portion p{};
+                bool clear = false;
+                while (piece.more()) {
+                    p = piece.portion(A);
+                    clear = piece.tile.n == 0 && p.first;
+                    if (p.work || clear) break;
+                    piece.advance(A);
+                }
+                const bool more = piece.more();
+                Unit u;
+                u.kind = !more ? kEnd : p.work ? kWork : kClear;
+                u.h = p.h; u.x0 = p.x0; u.x1 = p.x1;
+                u.direct = clear || p.whole;
+                u.tile = piece.tile;
+                if (more && !u.direct && p.x0 == 0) told = {piece.column * A.Hkv + p.h, piece.parts(A, blockIdx.x)};
+                const unsigned slot = walked % kUnitSlots;
+                if (walked >= (unsigned)kUnitSlots &&
+                    !warp_wait(bar_unitfree + 8 * slot, (walked / kUnitSlots - 1) & 1, abort_flag, P.wait_budget))
+                    break;
+                if (lane == 0) {
+                    reinterpret_cast<Unit*>(smem + C::kOffUnits)[slot] = u;
+                    mbar_arrive(bar_unit + 8 * slot);
+                }
+                __syncwarp();
+                if (!more) break;
+                piece.advance(A);
+            }
+            if (lane == 0) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
+        } else if (warp == 12) {
             // =====================================================================
             // MMA issue: the whole warp walks the units, the instructions execute on one elected lane.
             // =====================================================================
@@ -200,11 +264,12 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             unsigned fills = 0, units[2] = {0, 0}, tiles[2] = {0, 0};           // tiles of keys and values taken; units, tiles of each half
             unsigned queries = 0, seq = 0;                       // units; tiles of the CTA
             bool copied = false;                                 // rows of the tile whose keys came last were copied
-            for (; ok && piece.more(); piece.advance(A)) {
-                const Piece::Portion p = piece.portion(A);
-                if (!p.work) continue;
-                const int n = p.x1 - p.x0;
-                const bool two = SPLIT ? n > 1 : piece.tile.rows > kHalfRows;
+            for (unsigned walked = 0; ok;) {
+                const Unit u = next_unit(walked);
+                if (u.kind == kEnd) break;
+                if (u.kind != kWork) continue;
+                const int n = u.x1 - u.x0;
+                const bool two = SPLIT ? n > 1 : u.tile.rows > kHalfRows;
                 auto wait_full = [&]() { ok = ok && mbar_wait(bar_full + 8 * (fills % ST), (fills / ST) & 1, abort_flag, P.wait_budget); };
                 // The keys of the next tile have landed.  Rows that threads copied are ordinary writes, which the tensor cores see
                 // behind a proxy fence (some hundred cycles on the chain of every tile: not for those that TMA brought).
@@ -286,18 +351,18 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         if (copied) fence_async_smem();          // (still tile j's)
                         fills = v + 1;
                         if (more) wait_keys();
-                        auto half_of = [&](int half) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (half == 1 && !two) break;
                             wait_p(half, j == 0);
-                            if (!ok) return;
+                            if (!ok) break;
                             tc_fence_after();
                             fills = v;
                             weighted(half, j == 0);
                             if (!more) mma_commit_e(bar_o + 8 * half, leader);
                             fills = v + 1;
                             if (more) scores(half);
-                        };
-                        half_of(0);
-                        if (two && ok) half_of(1);
+                        }
                         if (!ok) break;
                         fills = v;
                         release();                               // V
@@ -327,10 +392,13 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             // A tile's keys: this thread's (the lt-th) page and slot, and where the keys and values of all of them are (elements).
             // runs: bit i is set where the run of A.align keys that key i * 16 belongs to is there as a whole.
             struct Keys { int page, slot; unsigned runs; const long long* at; };
-            for (; ok && piece.more(); piece.advance(A)) {
-                const Piece::Portion p = piece.portion(A);
-                if (!p.work) continue;
-                const Tile& x = piece.tile;
+            for (unsigned walked = 0;;) {
+                const Unit p = next_unit(walked);
+                if (p.kind == kEnd) ok = false;
+                ok = loaders_agree(ok);
+                if (!ok) break;
+                if (p.kind != kWork) continue;
+                const Tile& x = p.tile;
                 const int n = p.x1 - p.x0;
                 auto fill = [&](const CUtensorMap* map, const uint16_t* src, const Keys& k, int offset) {
                     const unsigned s = fills % ST;
@@ -415,28 +483,23 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     }
                     ++queries;
                 };
-                Keys k = keys_of(0);
-                if (!ok) break;
-                fill(&tmK, kc, k, 0);
-                load_queries();
-                for (int j = 0; j < n; ++j) {
-                    if constexpr (SPLIT) {                       // K0, K1, V0, K2, V1, ...
-                        Keys next{};
-                        if (j + 1 < n) {
-                            next = keys_of(j + 1);
-                            if (!ok) break;
-                            fill(&tmK, kc, next, 0);
-                        }
-                        fill(&tmV, vc, k, kKeys);
-                        k = next;
-                    } else {                                     // K0, V0, K1, V1, ...
-                        fill(&tmV, vc, k, kKeys);
-                        if (j + 1 < n) {
-                            k = keys_of(j + 1);
-                            if (!ok) break;
-                            fill(&tmK, kc, k, 0);
-                        }
+                // K0, V0, K1, V1, ...; with kSplit K0, K1, V0, K2, V1, ..., so that the keys are ahead of the other half's values
+                Keys keys{}, values{};
+#pragma unroll 1
+                for (int f = 0; f < 2 * n; ++f) {
+                    const bool is_key = SPLIT ? f == 0 || (f & 1 && f < 2 * n - 1) : !(f & 1);
+                    const int j = is_key ? (f + 1) / 2 : 0;
+                    if (is_key) {
+                        const Keys k = keys_of(j);
+                        if (!ok) break;
+                        values = SPLIT ? keys : k;
+                        if (SPLIT && n == 1) values = k;
+                        keys = k;
+                    } else if (SPLIT && f == 2 * n - 1) {
+                        values = keys;
                     }
+                    fill(is_key ? &tmK : &tmV, is_key ? kc : vc, is_key ? keys : values, is_key ? 0 : kKeys);
+                    if (f == 0) load_queries();
                 }
                 ok = loaders_agree(ok);                          // the places have been read by everyone
             }
@@ -455,15 +518,13 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         bool ok = !gave_up(abort_flag);
         unsigned mine = 0, seq = 0, units = 0, exchanges = 0;    // tiles of this half, tiles of the CTA, units of this half
         const uint64_t sc2 = pack2(A.scale_log2, A.scale_log2);
-        for (; ok && piece.more(); piece.advance(A)) {
-            const Piece::Portion p = piece.portion(A);
-            const Tile& x = piece.tile;
-            const bool clear = x.n == 0 && p.first;
-            if (!p.work && !clear) continue;
-            const int n = p.work ? p.x1 - p.x0 : 0;
-            const bool direct = clear || p.whole;
+        for (unsigned walked = 0; ok;) {
+            const Unit p = next_unit(walked);
+            if (p.kind == kEnd) break;
+            const Tile& x = p.tile;
+            const int n = p.kind == kWork ? p.x1 - p.x0 : 0;
+            const bool direct = p.direct;
             const int where = 2 * (int)blockIdx.x + (p.x0 == 0 ? 1 : 0);
-            if (!direct && p.x0 == 0) told = {piece.column * A.Hkv + p.h, piece.parts(A, blockIdx.x)};
             const bool active = SPLIT ? half == 0 || n > 1 : half == 0 || x.rows > kHalfRows;
             if (!active) {
                 seq += n;
@@ -569,83 +630,96 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         for (int pc = 0; pc < 4; ++pc) tmem_st16(scol + 16 * pc, pk[pc]);
                     }
                 }
+                // Other tiles, 64 columns at a time.
+                if (!stored) {
+                    auto bits_of = [&](int pc) {                 // the row's columns of 32 from 32 pc on
+                        const int t0 = base + 32 * pc;
+                        const uint32_t word = pc == 0 ? words[0] : pc == 1 ? words[1] : pc == 2 ? words[2] : words[3];
+                        return low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & word;
+                    };
 #pragma unroll 1
-                for (int pc = stored ? 4 : 0; pc < 4; ++pc) {
-                    const int t0 = base + 32 * pc;
-                    const uint32_t word = pc == 0 ? words[0] : pc == 1 ? words[1] : pc == 2 ? words[2] : words[3];
-                    uint32_t pk[16];
-                    if (t0 > t_most || (t0 + 31 < t_least && t_least - (t0 + 31) >= A.K)) {       // no row of the warp sees the piece
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) pk[i] = 0u;
-                        tmem_st16(scol + 16 * pc, pk);
-                        continue;
-                    }
-                    uint32_t s[32];
-                    tmem_ld32(scol + 32 * pc, s);
-                    const uint64_t by2 = landed(sc2);
-                    const float by = lo_of(by2);
-                    // every row of the warp that counts sees all of the piece
-                    const bool open = word == 0xffffffffu && t0 + 31 <= t_least && t_most - t0 < A.K;
-                    uint32_t bits = 0xffffffffu;
-                    if (!open) bits = low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & word;
-                    if (__any_sync(0xffffffffu, m == -CUDART_INF_F && bits != 0u)) {         // first columns that a row sees
+                    for (int pc = 0; pc < 4; ++pc) {             // rows that meet their first columns: their maximum
+                        const uint32_t bits = bits_of(pc);
+                        if (!__any_sync(0xffffffffu, m == -CUDART_INF_F && bits != 0u)) continue;
+                        uint32_t s[32];
+                        tmem_ld32(scol + 32 * pc, s);
+                        const float by = landed(A.scale_log2);
                         float top = -CUDART_INF_F;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * by);
                         if (m == -CUDART_INF_F) m = top;
                     }
-                    bool done = false;
-                    {
-                        const float shift = m == -CUDART_INF_F ? 0.f : -m;
-                        const uint64_t nb2 = pack2(shift, shift);
+#pragma unroll 1
+                    for (int hc = 0; hc < 2; ++hc) {
+                        const uint32_t lo = bits_of(2 * hc), hi = bits_of(2 * hc + 1);
+                        uint32_t pk[2][16];
+                        if (!__any_sync(0xffffffffu, (lo | hi) != 0u)) {         // no row of the warp sees any of them
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) pk[0][i] = 0u;
+                            tmem_st16(scol + 32 * hc, pk[0]);
+                            tmem_st16(scol + 32 * hc + 16, pk[0]);
+                            continue;
+                        }
+                        const float base_m = m == -CUDART_INF_F ? 0.f : m;
+                        uint32_t s[2][32];
+                        tmem_ld32(scol + 64 * hc, s[0]);
+                        tmem_ld32(scol + 64 * hc + 32, s[1]);
+                        const uint64_t by2 = landed(sc2), nb2 = pack2(-base_m, -base_m);
                         float sum_a = 0.f, sum_b = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t e = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), by2, nb2);
-                            float a = fast_exp2(lo_of(e)), b = fast_exp2(hi_of(e));
-                            if (!open) {                         // whatever a hidden score gave
-                                a = (bits >> (2 * i)) & 1u ? a : 0.f;
-                                b = (bits >> (2 * i + 1)) & 1u ? b : 0.f;
+                        for (int w2 = 0; w2 < 2; ++w2) {
+                            const uint32_t bits = w2 ? hi : lo;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t e = fma2(pack2(__uint_as_float(s[w2][2 * i]), __uint_as_float(s[w2][2 * i + 1])), by2, nb2);
+                                // whatever a hidden score gave
+                                const float a = (bits >> (2 * i)) & 1u ? fast_exp2(lo_of(e)) : 0.f;
+                                const float b = (bits >> (2 * i + 1)) & 1u ? fast_exp2(hi_of(e)) : 0.f;
+                                sum_a += a;
+                                sum_b += b;
+                                pk[w2][i] = cvt_pack<BF16>(a, b);
                             }
-                            sum_a += a;
-                            sum_b += b;
-                            pk[i] = cvt_pack<BF16>(a, b);
                         }
                         const float rs = sum_a + sum_b;
-                        if (!__any_sync(0xffffffffu, !(rs <= kGrowSum))) {
+                        if (__builtin_expect(!__any_sync(0xffffffffu, !(rs <= kGrowSum)), 1)) {
                             l += rs;
-                            done = true;
+                            tmem_st16(scol + 32 * hc, pk[0]);    // over columns of this thread's that have been read
+                            tmem_st16(scol + 32 * hc + 16, pk[1]);
+                            continue;
                         }
-                    }
-                    if (!done) {
-                        const float base_m = m == -CUDART_INF_F ? 0.f : m;
-                        float over = -CUDART_INF_F;
+                        // Rare: a score has outgrown the row's maximum (or is not a number).  16 columns at a time, from TMEM again.
+                        auto exponents = [&](int q, uint32_t (&e)[16]) {
+                            tmem_ld16(scol + 64 * hc + 16 * q, e);
+                            const float by = landed(A.scale_log2), from = m == -CUDART_INF_F ? 0.f : m;
+                            const uint32_t bits = (q < 2 ? lo : hi) >> (16 * (q & 1));
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float e = (bits >> i) & 1u ? fmaf(__uint_as_float(s[i]), by, -base_m) : -CUDART_INF_F;
-                            s[i] = __float_as_uint(e);
-                            over = fmaxf(over, e);
+                            for (int i = 0; i < 16; ++i)
+                                e[i] = __float_as_uint((bits >> i) & 1u ? fmaf(__uint_as_float(e[i]), by, -from) : -CUDART_INF_F);
+                        };
+                        float over = -CUDART_INF_F;
+#pragma unroll 1
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t e[16];
+                            exponents(q, e);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) over = fmaxf(over, __uint_as_float(e[i]));
                         }
                         const bool grow = over > kGrow;
-                        if (__any_sync(0xffffffffu, grow)) {
-                            rescale(grow, over, had_tiles, pc);
-                            if (grow) {
+                        if (__any_sync(0xffffffffu, grow)) rescale(grow, over, had_tiles, 2 * hc);
+#pragma unroll 1
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t e[16], w8[8];
+                            exponents(q, e);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - over);
+                            for (int i = 0; i < 8; ++i) {
+                                const float a = fast_exp2(__uint_as_float(e[2 * i])), b = fast_exp2(__uint_as_float(e[2 * i + 1]));
+                                l += a + b;
+                                w8[i] = cvt_pack<BF16>(a, b);
                             }
+                            tmem_st8(scol + 32 * hc + 8 * q, w8);
                         }
-                        float sum_a = 0.f, sum_b = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float a = fast_exp2(__uint_as_float(s[2 * i])), b = fast_exp2(__uint_as_float(s[2 * i + 1]));
-                            sum_a += a;
-                            sum_b += b;
-                            pk[i] = cvt_pack<BF16>(a, b);
-                        }
-                        l += sum_a + sum_b;
                     }
-                    tmem_st16(scol + 16 * pc, pk);               // over columns of this thread's that have been read
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -692,7 +766,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 4; ++i) rows4[i] = __shfl_sync(0xffffffffu, my_row, (lane & ~3) | i);
             const int piece4 = lane & 3;
-#pragma unroll
+#pragma unroll 1
             for (int part = 0; part < DH / 32; ++part) {
                 uint32_t o[32];
                 if (n > 0) {
@@ -752,7 +826,6 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 ++units;
             }
         }
-        if (tid == 0) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
     }
 
     if (*abort_flag) abort_grace_sleep();
