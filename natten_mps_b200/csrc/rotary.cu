@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 namespace natten {
@@ -69,11 +70,24 @@ __device__ __forceinline__ void sin_cos_pi(double x, double& s, double& c) { sin
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T x[VEC]; };
 
+// Nothing that is read is written by the kernel.
+template <typename V> __device__ __forceinline__ V fetch(const void* p)
+{
+    V v;
+    if constexpr (sizeof(V) == 16) {
+        const uint4 x = __ldg(static_cast<const uint4*>(p));
+        memcpy(&v, &x, 16);
+    } else {
+        v = *static_cast<const V*>(p);
+    }
+    return v;
+}
+
 // position of token `n` of the padded batch, and whether its sequence has it
 __device__ __forceinline__ long long position_of(const TurnArgs& A, long long n, int& b, int& i, bool& live)
 {
-    b = A.length > 0 ? static_cast<int>(n / A.length) : 0;
-    i = static_cast<int>(n - static_cast<long long>(b) * A.length);
+    b = A.by_length.div(static_cast<int>(n));
+    i = static_cast<int>(n) - b * A.length;
     if (!A.table) {
         live = true;
         return A.positions ? A.positions[b * A.pos_stride[0] + i * A.pos_stride[1]] : i;
@@ -178,8 +192,8 @@ __global__ void __launch_bounds__(kThreads) turn_kernel(const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < VEC; ++i) x.x[i] = y.x[i] = down<T>(acc(0));
         } else {
-            x = *reinterpret_cast<const V*>(src + a);
-            if (b >= 0) y = *reinterpret_cast<const V*>(src + b);
+            x = fetch<V>(src + a);
+            if (b >= 0) y = fetch<V>(src + b);
             if (turned) {
                 if constexpr (INTER && VEC > 1) {
                     const acc *cs = cosv + t * A.half + a / 2, *sn = sinv + t * A.half + a / 2;
@@ -224,6 +238,7 @@ bool vectors_fit(const TurnArgs& A, int dtype, bool interleaved)
 int launch_turn(TurnArgs& A, int dtype, bool interleaved, cudaStream_t stream)
 {
     if (A.tokens == 0) return NATTEN_OK;
+    if (A.tokens > 0x7fffffffll - kMaxTokens) return NATTEN_E_UNSUPPORTED;
     const bool vec = vectors_fit(A, dtype, interleaved);
     const int n = vec ? 16 / (int)width_of(dtype) : 1;
     A.pair_units = vec && interleaved ? 2 * A.half / n : A.half / n;
@@ -237,11 +252,11 @@ int launch_turn(TurnArgs& A, int dtype, bool interleaved, cudaStream_t stream)
     t = std::min<long long>({t, kMaxTokens, std::max<long long>(1, (32 << 10) / (long long)(2 * acc * std::max(1, A.half)))});
     A.per_block = (int)t;
     const size_t smem = 2 * acc * (size_t)A.per_block * A.half;
+    A.by_length = FastDiv((uint32_t)A.length);
     A.by_token = FastDiv(per_token);
     A.by_row = FastDiv(A.row_units);
     A.by_copy = FastDiv(std::max(1, A.copy_units));
     const long long blocks = (A.tokens + t - 1) / t;
-    if (blocks > 0x7fffffffll) return NATTEN_E_UNSUPPORTED;
     auto go = [&](auto type, auto width, auto inter) {
         using T = decltype(type);
         turn_kernel<T, decltype(width)::value, decltype(inter)::value><<<(unsigned)blocks, kThreads, smem, stream>>>(A);
@@ -287,6 +302,7 @@ int natten_rotary(const natten_rotary_params_t* p, const void* q, const void* k,
     TurnArgs A{};
     A.tokens = (long long)p->batch * p->length;
     if (A.tokens == 0) return NATTEN_OK;
+    if (A.tokens > 0x7fffffffll - kMaxTokens) return NATTEN_E_UNSUPPORTED;
     if (!q || !q_out || (k == nullptr) != (k_out == nullptr) || (p->rotary_dim > 0 && !p->frequencies)) return NATTEN_E_INVALID;
     A.q = q; A.k = k; A.q_out = q_out; A.k_out = k_out;
     A.freq = p->frequencies;
@@ -310,6 +326,7 @@ int natten_paged_append(const natten_paged_params_t* p, const void* q, const voi
     TurnArgs A{};
     A.tokens = (long long)p->batch * p->length;
     if (A.tokens == 0) return NATTEN_OK;
+    if (A.tokens > 0x7fffffffll - kMaxTokens) return NATTEN_E_UNSUPPORTED;
     if (!k || !v || !k_cache || !v_cache || (q == nullptr) != (q_out == nullptr) || !p->page_table || !p->cache_lens ||
         (p->rotary_dim > 0 && !p->frequencies))
         return NATTEN_E_INVALID;
