@@ -213,8 +213,8 @@ int natten_paged_append(const natten_paged_params_t* params, const void* q, cons
 /* out [B, L, Hq, D] = softmax(scale * q k^T) v over positions p, p - dilation, ..., p - (kernel - 1) * dilation
  * of the query's own sequence (those that are there), lse [B, L, Hq] float (or NULL) its log-sum-exp.  Rows
  * that see nothing and rows past seq_lens: out 0, lse -inf.  `workspace` holds the partial results of keys that
- * several CTAs share, natten_paged_workspace_bytes(params) bytes (16-byte aligned); it needs no initial value
- * and belongs to one call at a time.                                                                          */
+ * several CTAs share, natten_paged_workspace_bytes(params) bytes (16-byte aligned; 0: none is needed); it needs no
+ * initial value and belongs to one call at a time.                                                            */
 int natten_paged_fwd(const natten_paged_params_t* params, const void* q, const void* k_cache, const void* v_cache,
                      void* out, void* lse, void* workspace, size_t workspace_bytes, void* stream);
 size_t natten_paged_workspace_bytes(const natten_paged_params_t* params);

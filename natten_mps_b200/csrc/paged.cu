@@ -209,7 +209,10 @@ bool divide(Args& A, const Shape& shape)
 enum class Family { kGeneral, kWarp, kTc };
 struct Chosen { Args A; Family family; bool aligned; size_t workspace; };
 
-size_t workspace_of(const Args& A) { return (shared_bytes(A.ctas) + 2 * (size_t)A.ctas * slot_bytes(A.M, A.D) + 255) & ~(size_t)255; }
+size_t workspace_of(const Args& A)
+{
+    return A.whole ? 0 : (shared_bytes(A.ctas) + 2 * (size_t)A.ctas * slot_bytes(A.M, A.D) + 255) & ~(size_t)255;
+}
 
 int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void* kc, const void* vc)
 {
@@ -279,7 +282,7 @@ int natten_paged_fwd(const natten_paged_params_t* p, const void* q, const void* 
     Args& A = c.A;
     if (A.B == 0 || A.L == 0) return NATTEN_OK;
     if (!q || !out || !A.cache_lens || (A.table_width > 0 && !A.table) || (A.pages > 0 && (!k_cache || !v_cache))) return NATTEN_E_INVALID;
-    if (workspace_bytes < c.workspace || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return NATTEN_E_WORKSPACE;
+    if (c.workspace > 0 && (workspace_bytes < c.workspace || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))) return NATTEN_E_WORKSPACE;
     A.out = out;
     A.lse = static_cast<float*>(lse);
     A.ws = static_cast<unsigned char*>(workspace);

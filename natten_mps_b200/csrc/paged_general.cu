@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant
                 }
         }
     }
-    if (tid == 0) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
+    if (tid == 0 && !A.whole) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
 }
 
 } // namespace

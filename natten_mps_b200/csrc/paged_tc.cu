@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 if (!more) break;
                 piece.advance(A);
             }
-            if (lane == 0) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
+            if (lane == 0 && !A.whole) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
         } else if (warp == 12) {
             // =====================================================================
             // MMA issue: the whole warp walks the units, the instructions execute on one elected lane.

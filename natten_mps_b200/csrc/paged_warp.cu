@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
         }
         __syncthreads();                     // the exchange has been read
     }
-    if (tid == 0) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
+    if (tid == 0 && !A.whole) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
 }
 
 template <typename F> auto by_config(const Args& A, int M, F&& f)

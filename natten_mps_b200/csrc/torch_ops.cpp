@@ -489,8 +489,9 @@ std::tuple<Tensor, Tensor> paged_cuda(const Tensor& q_in, const Tensor& k_cache,
     p.dilation = (int)dilation;
     p.scale = scale;
     Tensor out = fresh(q.sizes(), q.scalar_type(), q), lse = fresh(q.sizes().slice(0, 3), at::kFloat, q);
-    const size_t ws_bytes = std::max<size_t>(natten_paged_workspace_bytes(&p), 256);
-    Tensor ws = fresh({(int64_t)ws_bytes}, at::kByte, q);
+    const size_t ws_bytes = natten_paged_workspace_bytes(&p);
+    Tensor ws;
+    if (ws_bytes) ws = fresh({(int64_t)ws_bytes}, at::kByte, q);
     poll_status(q);
     check(natten_paged_fwd(&p, ptr(q), k_cache.const_data_ptr(), v_cache.const_data_ptr(), out_ptr(out), out_ptr(lse), out_ptr(ws), ws_bytes,
                            stream_of(q)),
@@ -759,6 +760,11 @@ void no_backward(std::initializer_list<const Tensor*> tensors, const char* what)
     TORCH_CHECK(!wants_grad(tensors), "natten_b200: ", what, " has no backward pass (it serves a cache); call it under torch.no_grad() "
                 "or with detached tensors");
 }
+void written_in_place(std::initializer_list<const Tensor*> tensors)
+{
+    for (const Tensor* t : tensors)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 Tensor append_autograd(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
                        const Tensor& lens, const OptTensor& seq_lens, const OptTensor& query, const OptTensor& freq, bool interleaved,
                        double magnitude)
@@ -769,8 +775,7 @@ Tensor append_autograd(const Tensor& k, const Tensor& v, const Tensor& k_cache, 
         at::AutoDispatchBelowADInplaceOrView below;
         out = call_append(k, v, k_cache, v_cache, table, lens, seq_lens, query, freq, interleaved, magnitude);
     }
-    for (const Tensor* c : {&k_cache, &v_cache})
-        if (!c->is_inference()) c->unsafeGetTensorImpl()->bump_version();       // written in place
+    written_in_place({&k_cache, &v_cache});
     return out;
 }
 std::tuple<Tensor, Tensor> paged_autograd(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
@@ -1296,7 +1301,13 @@ PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n)
     Tensor out;
     {
         NoGil nogil;
-        out = call_append(*k, *v, *c.k, *c.v, *c.table, *c.lens, c.seq_lens, query, freq, interleaved, *magnitude);
+        if (wants_grad({k, v, c.k, c.v, opt_ptr(query), opt_ptr(freq)})) {
+            out = call_append(*k, *v, *c.k, *c.v, *c.table, *c.lens, c.seq_lens, query, freq, interleaved, *magnitude);      // raises
+        } else {                             // nothing for autograd to do but the version counters: one dispatch less
+            at::AutoDispatchBelowADInplaceOrView below;
+            out = call_append(*k, *v, *c.k, *c.v, *c.table, *c.lens, c.seq_lens, query, freq, interleaved, *magnitude);
+            written_in_place({c.k, c.v});
+        }
     }
     if (!query) Py_RETURN_NONE;
     return wrap(std::move(out));
@@ -1321,6 +1332,8 @@ PyObject* py_paged(PyObject*, PyObject* const* args, Py_ssize_t n)
     std::tuple<Tensor, Tensor> r;
     {
         NoGil nogil;
+        std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+        if (!wants_grad({q, c.k, c.v})) below.emplace();                 // (with gradients the autograd kernel raises)
         r = call_paged(*q, *c.k, *c.v, *c.table, *c.lens, c.seq_lens, kernel[0], dilation[0], *scale);
     }
     if (!want_lse) return wrap(std::move(std::get<0>(r)));
