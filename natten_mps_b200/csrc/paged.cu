@@ -207,7 +207,7 @@ bool divide(Args& A, const Shape& shape)
 }
 
 enum class Family { kGeneral, kWarp, kTc };
-struct Chosen { Args A; Family family; bool aligned; size_t workspace; };
+struct Chosen { Args A; Family family; bool aligned; int warps; size_t workspace; };
 
 size_t workspace_of(const Args& A)
 {
@@ -247,8 +247,14 @@ int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void*
     c.family = Family::kGeneral;
     c.workspace = workspace_of(general);
     const bool tc = !simt && tc_shape(p->dtype, A, p->dim % 8 == 0, shape);
-    if (tc || (!simt && warp_shape(p->dtype, A, p->dim % 8 == 0, shape))) {
+    c.warps = 8;
+    if (tc || (!simt && warp_shape(p->dtype, A, p->dim % 8 == 0, c.warps, shape))) {
         if (!divide(A, shape)) return NATTEN_E_UNSUPPORTED;
+        if (!tc && A.whole && (long long)A.columns * A.Hkv > sm_count()) {
+            c.warps = 4;
+            warp_shape(p->dtype, A, true, c.warps, shape);
+            divide(A, shape);
+        }
         c.workspace = std::max(c.workspace, workspace_of(A));
         if (c.aligned) c.family = tc ? Family::kTc : Family::kWarp;
     }
@@ -288,7 +294,7 @@ int natten_paged_fwd(const natten_paged_params_t* p, const void* q, const void* 
     A.ws = static_cast<unsigned char*>(workspace);
     const cudaStream_t s = (cudaStream_t)stream;
     note_path(c.family == Family::kTc ? NATTEN_PATH_TCGEN05 : c.family == Family::kWarp ? NATTEN_PATH_WARP : NATTEN_PATH_SIMT);
-    const int err = c.family == Family::kTc ? tc_run(p->dtype, A, s) : c.family == Family::kWarp ? warp_run(p->dtype, A, s)
+    const int err = c.family == Family::kTc ? tc_run(p->dtype, A, s) : c.family == Family::kWarp ? warp_run(p->dtype, A, c.warps, s)
                                                                                                : general_run(p->dtype, A, c.aligned, s);
     return err || A.whole ? err : join(p->dtype, A, s);
 }

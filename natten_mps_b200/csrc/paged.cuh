@@ -252,8 +252,8 @@ __device__ __forceinline__ bool locate(const Args& A, const Tile& x, int t, int&
 struct Shape { int M, keys, overhead, least, most, ctas; };
 bool general_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int general_run(int dtype, const Args& A, bool aligned, cudaStream_t s);
-bool warp_shape(int dtype, const Args& A, bool aligned, Shape& shape);
-int warp_run(int dtype, const Args& A, cudaStream_t s);
+bool warp_shape(int dtype, const Args& A, bool aligned, int warps, Shape& shape);
+int warp_run(int dtype, const Args& A, int warps, cudaStream_t s);
 bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape);
 int tc_run(int dtype, const Args& A, cudaStream_t s);
 

@@ -32,9 +32,9 @@ using tcplan::fast_exp2;
 
 namespace {
 
-// MT: tiles of 16 rows; DP: head dim rounded up to 32, 64, 128 or 256
-template <int DP, int MT> struct Cfg {
-    static constexpr int kWarps = DP == 256 ? 4 : 8, kThreads = 32 * kWarps;
+// MT: tiles of 16 rows; DP: head dim rounded up to 32, 64, 128 or 256; NW: warps of a CTA
+template <int DP, int MT, int NW> struct Cfg {
+    static constexpr int kWarps = NW, kThreads = 32 * kWarps, kPerSm = DP == 256 ? 1 : 8 / NW;
     static constexpr int kKeys = DP <= 64 ? 32 : 16;             // keys of a warp's step
     static constexpr int kStages = 3;
     static constexpr int kRowBytes = DP * 2, kChunks = DP / 8;   // 16-byte chunks of a row
@@ -63,10 +63,10 @@ template <int DP> __device__ __forceinline__ uint32_t at(int r, int c)
     return r * (DP * 2) + ((DP >= 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
 }
 
-template <int DP, int MT, bool BF16>
-__global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __grid_constant__ Args A)
+template <int DP, int MT, int NW, bool BF16>
+__global__ void __launch_bounds__(Cfg<DP, MT, NW>::kThreads, Cfg<DP, MT, NW>::kPerSm) warp_kernel(const __grid_constant__ Args A)
 {
-    using C = Cfg<DP, MT>;
+    using C = Cfg<DP, MT, NW>;
     constexpr int NK = C::kKeys, NT = NK / 8, ST = C::kStages, kWarps = C::kWarps, kThreads = C::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
     float2* sums = reinterpret_cast<float2*>(smem + C::kSums);
@@ -321,51 +321,60 @@ __global__ void __launch_bounds__(Cfg<DP, MT>::kThreads, 1) warp_kernel(const __
     if (tid == 0 && !A.whole) reinterpret_cast<Shared*>(A.ws)[blockIdx.x] = told;
 }
 
-template <typename F> auto by_config(const Args& A, int M, F&& f)
+// f(DP, MT, NW) for the call's head dim, rows of a tile and warps of a CTA
+template <typename F> auto by_config(const Args& A, int M, int warps, F&& f)
 {
-    auto rows = [&](auto dp) {
+    auto by_warps = [&](auto dp, auto mt) {
         constexpr int kDim = decltype(dp)::value;
         if constexpr (kDim < 256) {
-            if (M == 32) return f(dp, std::integral_constant<int, 2>{});
+            if (warps == 8) return f(dp, mt, std::integral_constant<int, 8>{});
         }
-        return f(dp, std::integral_constant<int, 1>{});
+        return f(dp, mt, std::integral_constant<int, 4>{});
     };
-    if (A.D <= 32) return rows(std::integral_constant<int, 32>{});
-    if (A.D <= 64) return rows(std::integral_constant<int, 64>{});
-    if (A.D <= 128) return rows(std::integral_constant<int, 128>{});
-    return rows(std::integral_constant<int, 256>{});
+    auto by_rows = [&](auto dp) {
+        constexpr int kDim = decltype(dp)::value;
+        if constexpr (kDim < 256) {
+            if (M == 32) return by_warps(dp, std::integral_constant<int, 2>{});
+        }
+        return by_warps(dp, std::integral_constant<int, 1>{});
+    };
+    if (A.D <= 32) return by_rows(std::integral_constant<int, 32>{});
+    if (A.D <= 64) return by_rows(std::integral_constant<int, 64>{});
+    if (A.D <= 128) return by_rows(std::integral_constant<int, 128>{});
+    return by_rows(std::integral_constant<int, 256>{});
 }
 
 } // namespace
 
-bool warp_shape(int dtype, const Args& A, bool aligned, Shape& shape)
+// `warps`: 8 (one CTA an SM) or 4 (two).
+bool warp_shape(int dtype, const Args& A, bool aligned, int warps, Shape& shape)
 {
     if ((dtype != NATTEN_F16 && dtype != NATTEN_BF16) || !aligned || A.D > 256) return false;
     // 16 rows, or 32 where a class has more (256 channels of 32 rows do not fit the registers)
     const long long rows = ((long long)A.L + A.dil - 1) / A.dil * A.G;
     shape.M = rows > 16 && A.D <= 128 ? 32 : 16;
-    by_config(A, shape.M, [&](auto dp, auto mt) {
-        using C = Cfg<decltype(dp)::value, decltype(mt)::value>;
+    by_config(A, shape.M, warps, [&](auto dp, auto mt, auto nw) {
+        using C = Cfg<decltype(dp)::value, decltype(mt)::value, decltype(nw)::value>;
         shape.keys = C::kWarps * C::kKeys;
-        shape.ctas = sm_count();
+        shape.ctas = C::kPerSm * sm_count();
+        shape.most = 64 / C::kWarps;
     });
     shape.overhead = 1;
     shape.least = 2;
-    shape.most = 8;
     return true;
 }
 
-int warp_run(int dtype, const Args& A, cudaStream_t s)
+int warp_run(int dtype, const Args& A, int warps, cudaStream_t s)
 {
-    return by_config(A, A.M, [&](auto dp, auto mt) {
-        using C = Cfg<decltype(dp)::value, decltype(mt)::value>;
+    return by_config(A, A.M, warps, [&](auto dp, auto mt, auto nw) {
+        using C = Cfg<decltype(dp)::value, decltype(mt)::value, decltype(nw)::value>;
         cudaError_t err;
         auto go = [&](auto* kernel) {
             err = ensure_dynamic_smem((const void*)kernel, C::kSmem);
             if (err == cudaSuccess) kernel<<<A.ctas, C::kThreads, C::kSmem, s>>>(A);
         };
-        if (dtype == NATTEN_BF16) go(warp_kernel<decltype(dp)::value, decltype(mt)::value, true>);
-        else go(warp_kernel<decltype(dp)::value, decltype(mt)::value, false>);
+        if (dtype == NATTEN_BF16) go(warp_kernel<decltype(dp)::value, decltype(mt)::value, decltype(nw)::value, true>);
+        else go(warp_kernel<decltype(dp)::value, decltype(mt)::value, decltype(nw)::value, false>);
         if (err == cudaSuccess) err = cudaGetLastError();
         simt_count_launch(1);
         return (int)err;
