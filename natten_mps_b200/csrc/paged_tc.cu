@@ -766,7 +766,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 4; ++i) rows4[i] = __shfl_sync(0xffffffffu, my_row, (lane & ~3) | i);
             const int piece4 = lane & 3;
-#pragma unroll 1
+            constexpr int kPartsAtOnce = SPLIT ? 1 : DH / 32;    // (joining two halves, the code is too long to unroll)
+#pragma unroll kPartsAtOnce
             for (int part = 0; part < DH / 32; ++part) {
                 uint32_t o[32];
                 if (n > 0) {
