@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             if (!in_tile) index = -1;
             const int t_least = __reduce_min_sync(0xffffffffu, live ? tq : 0x7fffffff), t_most = __reduce_max_sync(0xffffffffu, live ? tq : -1);
             if (!live) tq = -1;
-            float m = -CUDART_INF_F, l = 0.f;
+            float m = tq >= 0 ? -CUDART_INF_F : 0.f, l = 0.f;    // (rows that do not count hold no tile up)
             // rare: a score far above the maximum.  Move it; rescale O (its products so far are done, see bar_s), the sum and the
             // probabilities of this tile's first `pieces` pieces.
             auto rescale = [&](bool grow, float over, bool had_tiles, int pieces) {
@@ -590,19 +590,40 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
+                auto bits_of = [&](int pc) {                     // the row's columns of 32 from 32 pc on
+                    const int t0 = base + 32 * pc;
+                    const uint32_t word = pc == 0 ? words[0] : pc == 1 ? words[1] : pc == 2 ? words[2] : words[3];
+                    return low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & word;
+                };
+                if (__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
+#pragma unroll 1
+                    for (int pc = 0; pc < 4; ++pc) {             // rows that meet their first columns: their maximum
+                        const uint32_t bits = bits_of(pc);
+                        if (!__any_sync(0xffffffffu, m == -CUDART_INF_F && bits != 0u)) continue;
+                        uint32_t s[32];
+                        tmem_ld32(scol + 32 * pc, s);
+                        const float by = landed(A.scale_log2);
+                        float top = -CUDART_INF_F;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * by);
+                        if (m == -CUDART_INF_F) m = top;
+                    }
+                }
                 // A tile that every row of the warp sees all of (most of a long context): no masks, and the probabilities stay in
                 // registers until the tile's sum has told that none of them outgrew its maximum.
                 bool stored = false;
                 if ((words[0] & words[1] & words[2] & words[3]) == 0xffffffffu && base + kKeys - 1 <= t_least && t_most - base < A.K &&
                     !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
-                    uint32_t s[4][32], pk[4][16];                // all columns at once: one wait, and nothing drains in between
+                    uint32_t s[4][32], pk[4][16];                // two pieces ahead: all four at once would spill
                     const uint64_t nb2 = pack2(-m, -m);
                     uint64_t sum0 = 0ull, sum1 = 0ull;
-#pragma unroll
-                    for (int pc = 0; pc < 4; ++pc) tmem_ld32(scol + 32 * pc, s[pc]);
-                    const uint64_t by2 = landed(sc2);
+                    tmem_ld32(scol, s[0]);
+                    tmem_ld32(scol + 32, s[1]);
+                    uint64_t by2 = landed(sc2);
 #pragma unroll
                     for (int pc = 0; pc < 4; ++pc) {
+                        if (pc < 2) tmem_ld32(scol + 32 * (pc + 2), s[pc + 2]);
                         uint32_t(&x)[32] = s[pc];
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
@@ -620,6 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             pk[pc][i] = cvt_pack<BF16>(a, b);
                             pk[pc][i + 1] = cvt_pack<BF16>(c, d);
                         }
+                        if (pc < 2) by2 = landed(by2);
                     }
                     sum0 = add2(sum0, sum1);
                     const float rs = lo_of(sum0) + hi_of(sum0);
@@ -632,24 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 }
                 // Other tiles, 64 columns at a time.
                 if (!stored) {
-                    auto bits_of = [&](int pc) {                 // the row's columns of 32 from 32 pc on
-                        const int t0 = base + 32 * pc;
-                        const uint32_t word = pc == 0 ? words[0] : pc == 1 ? words[1] : pc == 2 ? words[2] : words[3];
-                        return low_bits(tq - t0 + 1) & ~(tq - t0 >= A.K ? low_bits(tq - t0 - A.K + 1) : 0u) & word;
-                    };
-#pragma unroll 1
-                    for (int pc = 0; pc < 4; ++pc) {             // rows that meet their first columns: their maximum
-                        const uint32_t bits = bits_of(pc);
-                        if (!__any_sync(0xffffffffu, m == -CUDART_INF_F && bits != 0u)) continue;
-                        uint32_t s[32];
-                        tmem_ld32(scol + 32 * pc, s);
-                        const float by = landed(A.scale_log2);
-                        float top = -CUDART_INF_F;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * by);
-                        if (m == -CUDART_INF_F) m = top;
-                    }
 #pragma unroll 1
                     for (int hc = 0; hc < 2; ++hc) {
                         const uint32_t lo = bits_of(2 * hc), hi = bits_of(2 * hc + 1);

@@ -269,3 +269,29 @@ def test_missing_pages(L, Hq, Hkv, page, D, kernel):
             table[b, n] = (-1, 10 ** 9)[n % 2]
     out, _ = _check((q, k_cache, v_cache, table, lens, new), kernel, 1)
     assert not bool(out.isnan().any())
+
+
+@pytest.mark.parametrize("lens,new,L,Hq,Hkv,D,page,kernel,dilation", [
+    ([700], [300], 300, 8, 2, 64, 16, 40, 1),          # several row tiles a sequence, windows shorter than a tile of keys
+    ([520, 300], [300, 171], 300, 4, 1, 128, 64, None, 1),
+    ([90, 333], [70, 70], 70, 12, 4, 64, 16, None, 1),  # a group that no row tile holds a whole number of
+    ([333, 90], [70, 61], 70, 6, 2, 128, 24, 100, 1),
+    ([400], [200], 200, 4, 2, 64, 32, 300, 2),
+], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_several_row_tiles(dtype, lens, new, L, Hq, Hkv, D, page, kernel, dilation):
+    _check(_problem(dtype, lens, new, L, Hq, Hkv, D, page), kernel, dilation)
+    assert _cabi.last_path() == "tcgen05"
+
+
+@pytest.mark.parametrize("dtype,L", [(BF16, 1), (BF16, 40), (BF16, 70), (F32, 3)])
+def test_what_is_not_finite_shows(dtype, L):
+    """A NaN or Inf in a key or value that the newest query sees reaches it; sequences and heads next to it stay as they were."""
+    for tensor, value in ((1, math.nan), (2, math.nan), (2, math.inf)):
+        p = list(_problem(dtype, [300, 200], [L, L], L, 4, 2, 64, 16, poison=False))
+        q, k_cache, v_cache, table, lens, new = p
+        clean = F.na1d_paged(*[t.cuda() for t in (q, k_cache, v_cache, table, lens)], return_lse=False)
+        p[tensor][table[0, 3], 5, 1] = value             # sequence 0, position 53, head 1
+        out = F.na1d_paged(*[t.cuda() for t in (q, p[1], p[2], table, lens)])
+        assert not bool(torch.isfinite(out[0, -1, 2:]).any())
+        assert torch.equal(out[1], clean[1]) and torch.equal(out[0, :, :2], clean[0, :, :2])
