@@ -7,6 +7,12 @@
 // its own maximum, and accumulates all channels of its weighted sum in registers.  Nothing in the loop waits for another warp.
 // At the end of the unit the warps' partial results are joined through shared memory.
 //
+// Measured on one B200, bf16, 16 heads of 128 on 4: one token for each of 64 sequences of 2048 - 16384 tokens 192 us (6.3 TB/s with the
+// join, 96 % of a copy); 8 sequences through a window of 255 7.7 us, where lengths, page table, first keys and the join of the warps
+// follow each other.  Eight warps a CTA or four and two CTAs an SM: with more short units than SMs two CTAs fill each other's
+// beginnings and ends (128 sequences, window 512: 31 us against 37.5), with fewer the unit's keys want all warps (32 sequences of
+// 512: 10.4 against 14.3).
+//
 // A key that no row of the unit sees (behind the last query, in front of the first window, on a page that is not there) is not
 // fetched: its line of shared memory is zero.  One that some rows see and others do not is multiplied by a weight of zero in those,
 // so there a NaN or Inf value reaches them, too.

@@ -8,7 +8,9 @@
 // keep their accuracy; the cosine and sine of what is left in 32), and then streams all heads of q, k and v, 16 bytes of each
 // half of a pair at a time.
 //
-// Bound by memory: 6 operations a pair against 8 bytes (16 bits).
+// Bound by memory in principle (6 operations a pair against 8 bytes in 16 bits); measured on one B200, 2 x 8191 tokens of 16 + 4 heads
+// of 128, bf16: 36 us a direction, 4.7 TB/s of 6.5, with 55 - 60 % of the issue slots taken.  One token
+// for each of 64 sequences: 3.5 us in a graph.  Other shapes of it were slower: a thread that keeps a channel's angles and walks the heads 53 us a direction, four units under way a thread 70, rows across threadIdx.y 37.
 #include "../../include/natten_b200.h"
 
 #include "device_cache.cuh"
