@@ -141,7 +141,8 @@ class _Rotary:
 
     def on(self, device) -> torch.Tensor:
         if device not in self._placed:
-            self._placed[device] = self.values.to(device)
+            with torch.inference_mode(False):              # kept for training, too, wherever the first call was
+                self._placed[device] = self.values.to(device)
         return self._placed[device]
 
 

@@ -175,3 +175,10 @@ def test_module_refusals():
     with pytest.raises(ValueError, match="rotary_dim"):
         nb.NeighborhoodAttention1D(32, 4, 3, rotary_dim=10)
     assert not any("freq" in name for name in m.state_dict())      # interchangeable with modules without positions
+
+
+def test_frequencies_first_placed_in_inference_mode_serve_training():
+    m = nb.NeighborhoodAttention1D(32, 4, 3, is_causal=True, rotary_dim=8)
+    with torch.inference_mode():
+        m._rotary.on(torch.device("meta"))
+    assert not m._rotary.on(torch.device("meta")).is_inference()
