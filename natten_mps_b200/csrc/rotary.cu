@@ -329,12 +329,14 @@ int natten_paged_append(const natten_paged_params_t* p, const void* q, const voi
     A.tokens = (long long)p->batch * p->length;
     if (A.tokens == 0) return NATTEN_OK;
     if (A.tokens > 0x7fffffffll - kMaxTokens) return NATTEN_E_UNSUPPORTED;
-    if (!k || !v || !k_cache || !v_cache || (q == nullptr) != (q_out == nullptr) || !p->page_table || !p->cache_lens ||
-        (p->rotary_dim > 0 && !p->frequencies))
+    if (!k || !v || (p->pages > 0 && (!k_cache || !v_cache)) || (q == nullptr) != (q_out == nullptr) ||
+        (p->table_width > 0 && !p->page_table) || !p->cache_lens || (p->rotary_dim > 0 && !p->frequencies))
         return NATTEN_E_INVALID;
     A.q = q; A.k = k; A.v = v; A.q_out = q_out; A.k_out = k_cache; A.v_out = v_cache;
     A.freq = p->frequencies;
-    A.table = p->page_table; A.cache_lens = p->cache_lens; A.seq_lens = p->seq_lens; A.table_stride = p->table_stride;
+    // A table without entries is not read, but tells the append from the rotation alone.
+    A.table = p->table_width > 0 ? p->page_table : p->cache_lens;
+    A.cache_lens = p->cache_lens; A.seq_lens = p->seq_lens; A.table_stride = p->table_stride;
     for (int i = 0; i < 3; ++i) {
         A.qs[i] = p->q_stride[i]; A.ks[i] = p->k_stride[i]; A.vs[i] = p->v_stride[i];
         A.kd[i] = p->k_cache_stride[i]; A.vd[i] = p->v_cache_stride[i];

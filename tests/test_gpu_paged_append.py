@@ -145,3 +145,17 @@ def test_refuses_gradients_and_writes_in_place():
         F.na1d_append(k.detach(), k.detach(), cache, cache, table, lens.cpu())
     with pytest.raises(ValueError, match="dtype"):
         F.na1d_append(k.detach(), k.detach(), cache.half(), cache.half(), table, lens)
+
+
+@pytest.mark.parametrize("pages,width", [(0, 2), (3, 0), (0, 0)])
+def test_no_pages(pages, width):
+    """Tokens without a page are dropped where no page is there at all; the query is rotated all the same."""
+    k, v, q = [_normal(i, 2, 3, 2, 64, dtype=torch.float32).cuda() for i in (1, 2, 3)]
+    cache = [torch.full((pages, 4, 2, 64), 7.0, device="cuda") for _ in range(2)]
+    table, lens = torch.zeros(2, width, dtype=torch.int32, device="cuda"), torch.tensor([3, 5]).int().cuda()
+    freq = rotary_frequencies(64)[0].cuda()
+    got = F.na1d_append(k, v, *cache, table, lens, query=q, frequencies=freq)
+    positions = torch.tensor([[0, 1, 2], [2, 3, 4]]).cuda()
+    assert torch.equal(got, F.na1d_rotary(q, k, freq, positions)[0])
+    assert all(bool((c == 7).all()) for c in cache)
+    assert not bool((F.na1d_paged(q, *cache, table, lens, 3) != 0).any())
