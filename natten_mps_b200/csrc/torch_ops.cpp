@@ -10,6 +10,7 @@
 // NotImplemented; functional.py then takes its own path, which raises the errors and serves the rare forms.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -370,6 +371,11 @@ Tensor as_index(const Tensor& t)
     const Tensor n = t.scalar_type() == at::kInt ? t : t.clamp(-1, 2147483647).to(at::kInt);
     return n.dim() == 0 || n.stride(-1) == 1 ? n : n.contiguous();
 }
+void in_31_bits(std::initializer_list<const Tensor*> tensors)
+{
+    for (const Tensor* t : tensors)
+        for (const int64_t n : t->sizes()) TORCH_CHECK_VALUE(n <= 2147483647, "natten_b200: a size of ", n, " is not supported");
+}
 void copy_strides(const Tensor& t, int64_t (&s)[3])      // [., ., heads, dim] with adjacent channels
 {
     for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
@@ -382,6 +388,7 @@ std::tuple<Tensor, Tensor> rotary_cuda(const Tensor& q_in, const Tensor& k_in, c
     require_cuda({&q_in, &k_in, &freq_in, &pos}, q_in);
     same_dtype(q_in, {&k_in});
     TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && freq_in.dim() == 1, "natten_b200: na1d_rotary takes [B, L, H, D] tensors");
+    in_31_bits({&q_in, &k_in});
     natten_rotary_params_t p{};
     const c10::cuda::CUDAGuard guard(q_in.device());
     const Tensor q = strided_input(q_in, 1, p.q_stride), k = strided_input(k_in, 1, p.k_stride), freq = as(freq_in, at::kDouble);
@@ -419,7 +426,7 @@ void paged_params(natten_paged_params_t& p, const Tensor& like, int64_t heads_q,
                       "natten_b200: shapes of new tokens, caches, page table and lengths do not match");
     for (const Tensor* c : {&k_cache, &v_cache})
         TORCH_CHECK_VALUE(c->size(3) == 1 || c->stride(3) == 1 || c->numel() == 0, "natten_b200: a cache's channels must be adjacent in memory");
-    TORCH_CHECK_VALUE(k_cache.size(0) <= 2147483647 && k_cache.size(1) <= 2147483647, "natten_b200: too many pages");
+    in_31_bits({&like, &k_cache, &table});
     held[0] = as_index(table);
     held[1] = as_index(lens);
     if (fresh_lens.defined()) held[2] = as_index(fresh_lens);
@@ -452,6 +459,8 @@ Tensor append_cuda(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache
     const c10::cuda::CUDAGuard guard(k_in.device());
     natten_paged_params_t p{};
     Tensor held[3], q, q_out, freq;
+    for (const Tensor* c : {&k_cache, &v_cache}) at::assert_no_internal_overlap(*c);
+    if (q_in.defined()) in_31_bits({&q_in});
     paged_params(p, k_in, q_in.defined() ? q_in.size(2) : 1, k_cache, v_cache, table, lens, fresh_lens, held);
     TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.size(2) == k_cache.size(2), "natten_b200: key, value and cache do not match");
     const Tensor k = strided_input(k_in, 1, p.k_stride), v = strided_input(v_in, 1, p.v_stride);

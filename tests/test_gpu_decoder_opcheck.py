@@ -52,3 +52,16 @@ def test_under_the_compiler():
     ref = F.na1d_rotary(x2, y2, freq)
     want = torch.autograd.grad(ref[0].sum() + (ref[1] * 3).sum(), [x2, y2])
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_refuses_sizes_past_31_bits_and_caches_that_overlap_themselves():
+    long = torch.zeros(1, 1, 1, 64, device="cuda").expand(1, 2 ** 32 + 5, 1, 64)         # refused before anything is made of it
+    cache = torch.zeros(4, 4, 1, 64, device="cuda")
+    table, lens, freq = torch.arange(4).int().view(1, 4).cuda(), torch.tensor([2]).int().cuda(), torch.ones(32).double().cuda()
+    for call in (lambda: F.na1d_rotary(long, long, freq), lambda: F.na1d_append(long, long, cache, cache.clone(), table, lens),
+                 lambda: F.na1d_paged(long, cache, cache, table, lens, 3)):
+        with pytest.raises(ValueError, match="not supported"):
+            call()
+    k = torch.zeros(1, 2, 1, 64, device="cuda")
+    with pytest.raises(RuntimeError):
+        F.na1d_append(k, k, cache[:1].expand(4, 4, 1, 64), cache, table, lens)
