@@ -587,6 +587,10 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 if (SPLIT && (j & 1) != half) continue;
                 const int base = x.base + (p.x0 + j) * kKeys;
                 const unsigned w = seq % kWordSlots;
+                // A half that took no part in the units before may be here long before this tile's words are: its barrier would be
+                // two phases behind, and one bit of phase cannot tell that from done.  So the first tile of a unit waits for its
+                // scores first (they are issued behind the words); from then on the words of tile seq - 16 are known to be past.
+                if (!had_tiles) ok = ok && mbar_wait(bar_s + 8 * half, mine & 1, abort_flag, P.wait_budget);
                 ok = ok && mbar_wait(bar_words + 8 * w, (seq / kWordSlots) & 1, abort_flag, P.wait_budget);
                 const volatile uint32_t* there_words = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffWords) + 4 * w;
                 const uint32_t words[4] = {there_words[0], there_words[1], there_words[2], there_words[3]};
