@@ -139,19 +139,45 @@ LIB.define("na1d_paged(Tensor query, Tensor key_cache, Tensor value_cache, Tenso
            "Tensor? seq_lens, int kernel_size, int dilation, float scale) -> (Tensor, Tensor)")
 
 
+def _same_tokens(a, b) -> bool:
+    return a.ndim == 4 and b.ndim == 4 and a.shape[:2] == b.shape[:2] and a.shape[3] == b.shape[3]
+
+
+def _check_pairs(frequencies, dim) -> None:
+    if frequencies is not None and (frequencies.ndim != 1 or 2 * frequencies.shape[0] > dim):
+        raise ValueError("natten_b200: frequencies are one for each rotated channel pair, at most D / 2.")
+
+
+def _check_caches(like, key_cache, value_cache, page_table, cache_lens, seq_lens) -> None:
+    lens_ok = all(t is None or tuple(t.shape) == tuple(like.shape[:1]) for t in (cache_lens, seq_lens))
+    if (like.ndim != 4 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape or key_cache.shape[3] != like.shape[3]
+            or page_table.ndim != 2 or page_table.shape[0] != like.shape[0] or not lens_ok):
+        raise ValueError("natten_b200: shapes of new tokens, caches, page table and lengths do not match.")
+
+
 @torch.library.impl(LIB, "na1d_rotary", "Meta")
 def _na1d_rotary_meta(query, key, frequencies, positions, interleaved, magnitude, inverse):
+    if not _same_tokens(query, key):
+        raise ValueError("natten_b200: na1d_rotary takes [B, L, H, D] tensors of the same B, L and D.")
+    _check_pairs(frequencies, query.shape[3])
     return query.new_empty(query.shape), key.new_empty(key.shape)
 
 
 @torch.library.impl(LIB, "na1d_append", "Meta")
 def _na1d_append_meta(key, value, key_cache, value_cache, page_table, cache_lens, seq_lens, query, frequencies,
                       interleaved, magnitude):
+    _check_caches(key, key_cache, value_cache, page_table, cache_lens, seq_lens)
+    if key.shape != value.shape or key.shape[2] != key_cache.shape[2]:
+        raise ValueError("natten_b200: key, value and cache do not match.")
+    if query is not None and not _same_tokens(query, key):
+        raise ValueError("natten_b200: na1d_append's query is [B, L, Hq, D] with key's B, L and D.")
+    _check_pairs(frequencies, key.shape[3])
     return key.new_empty(0 if query is None else query.shape)
 
 
 @torch.library.impl(LIB, "na1d_paged", "Meta")
 def _na1d_paged_meta(query, key_cache, value_cache, page_table, cache_lens, seq_lens, kernel_size, dilation, scale):
+    _check_caches(query, key_cache, value_cache, page_table, cache_lens, seq_lens)
     return query.new_empty(query.shape), query.new_empty(query.shape[:-1], dtype=torch.float32)
 
 

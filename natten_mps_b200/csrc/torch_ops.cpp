@@ -376,6 +376,11 @@ void in_31_bits(std::initializer_list<const Tensor*> tensors)
     for (const Tensor* t : tensors)
         for (const int64_t n : t->sizes()) TORCH_CHECK_VALUE(n <= 2147483647, "natten_b200: a size of ", n, " is not supported");
 }
+// [B, L, heads, D] with the same B, L and D
+bool same_tokens(const Tensor& a, const Tensor& b)
+{
+    return a.dim() == 4 && b.dim() == 4 && a.size(0) == b.size(0) && a.size(1) == b.size(1) && a.size(3) == b.size(3);
+}
 void copy_strides(const Tensor& t, int64_t (&s)[3])      // [., ., heads, dim] with adjacent channels
 {
     for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
@@ -387,7 +392,8 @@ std::tuple<Tensor, Tensor> rotary_cuda(const Tensor& q_in, const Tensor& k_in, c
     Tensor pos = positions.value_or(Tensor());
     require_cuda({&q_in, &k_in, &freq_in, &pos}, q_in);
     same_dtype(q_in, {&k_in});
-    TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && freq_in.dim() == 1, "natten_b200: na1d_rotary takes [B, L, H, D] tensors");
+    TORCH_CHECK_VALUE(same_tokens(q_in, k_in) && freq_in.dim() == 1 && freq_in.numel() <= q_in.size(3) / 2,
+                      "natten_b200: na1d_rotary takes [B, L, H, D] tensors of the same B, L and D and at most D / 2 frequencies");
     in_31_bits({&q_in, &k_in});
     natten_rotary_params_t p{};
     const c10::cuda::CUDAGuard guard(q_in.device());
@@ -460,9 +466,14 @@ Tensor append_cuda(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache
     natten_paged_params_t p{};
     Tensor held[3], q, q_out, freq;
     for (const Tensor* c : {&k_cache, &v_cache}) at::assert_no_internal_overlap(*c);
-    if (q_in.defined()) in_31_bits({&q_in});
+    if (q_in.defined()) {
+        TORCH_CHECK_VALUE(same_tokens(q_in, k_in), "natten_b200: na1d_append's query is [B, L, Hq, D] with key's B, L and D");
+        in_31_bits({&q_in});
+    }
     paged_params(p, k_in, q_in.defined() ? q_in.size(2) : 1, k_cache, v_cache, table, lens, fresh_lens, held);
     TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.size(2) == k_cache.size(2), "natten_b200: key, value and cache do not match");
+    TORCH_CHECK_VALUE(!freq_in.defined() || (freq_in.dim() == 1 && freq_in.numel() <= k_in.size(3) / 2),
+                      "natten_b200: na1d_append takes at most D / 2 frequencies");
     const Tensor k = strided_input(k_in, 1, p.k_stride), v = strided_input(v_in, 1, p.v_stride);
     if (q_in.defined()) {
         q = strided_input(q_in, 1, p.q_stride);
