@@ -596,8 +596,16 @@ std::optional<double> saved_scale(const AutogradContext* ctx)
     const c10::IValue& s = ctx->saved_data.at("s");
     return s.isNone() ? std::nullopt : std::optional<double>(s.toDouble());
 }
+// No operator here has a rule for forward-mode tangents, and what runs below autograd would drop them.
+void no_tangents(std::initializer_list<const Tensor*> tensors)
+{
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(),
+                                    "natten_b200: forward-mode derivatives (a Jacobian-vector product) are not implemented; use reverse mode");
+}
 bool wants_grad(std::initializer_list<const Tensor*> tensors)
 {
+    no_tangents(tensors);
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : tensors)
         if (t && t->defined() && t->requires_grad()) return true;

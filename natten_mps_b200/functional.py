@@ -439,8 +439,8 @@ def na1d_rotary(query, key, frequencies: torch.Tensor, positions: Optional[torch
 
     ``frequencies`` (float64, see ``rotary_frequencies``) and ``positions`` (int64 or int32, ``[L]`` or ``[B, L]``;
     default ``0 ... L - 1``) are on the device and carry no gradient.  A pair is channels ``(i, i + n)`` of the ``n``
-    frequencies, or ``(2i, 2i + 1)`` when ``interleaved``.  Differentiable (any number of times) in query and key;
-    float32, float16, bfloat16 and float64, computed in float32 (float64) and rounded once."""
+    frequencies, or ``(2i, 2i + 1)`` when ``interleaved``.  Differentiable (any number of times, in reverse mode) in
+    query and key; float32, float16, bfloat16 and float64, computed in float32 (float64) and rounded once."""
     if not torch.compiler.is_compiling():
         result = native.na_rotary(query, key, frequencies, positions, interleaved, magnitude)
         if result is not NotImplemented:
