@@ -465,7 +465,13 @@ Tensor append_cuda(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache
     const c10::cuda::CUDAGuard guard(k_in.device());
     natten_paged_params_t p{};
     Tensor held[3], q, q_out, freq;
-    for (const Tensor* c : {&k_cache, &v_cache}) at::assert_no_internal_overlap(*c);
+    // Everything is read and written in one launch, in no order.
+    for (const Tensor* c : {&k_cache, &v_cache}) {
+        at::assert_no_internal_overlap(*c);
+        for (const Tensor* t : {&k_in, &v_in, &q_in})
+            if (t->defined()) at::assert_no_overlap(*c, *t);
+    }
+    at::assert_no_overlap(k_cache, v_cache);
     if (q_in.defined()) {
         TORCH_CHECK_VALUE(same_tokens(q_in, k_in), "natten_b200: na1d_append's query is [B, L, Hq, D] with key's B, L and D");
         in_31_bits({&q_in});

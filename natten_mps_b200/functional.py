@@ -468,7 +468,8 @@ def na1d_append(key, value, key_cache, value_cache, page_table: torch.Tensor, ca
     ones, ``seq_lens [B]`` how many of the ``L`` rows are new tokens (default: all): new token ``i`` goes to position
     ``cache_lens - seq_lens + i``.  All three stay on the device (int32; int64 costs a conversion), so nothing is checked
     against them on the host: a token whose position has no page (a negative or too large table entry, a position past the
-    table) is dropped, and the rest of the cache is left as it was.  Pages that are written to must belong to one sequence.
+    table) is dropped, and the rest of the cache is left as it was.  Pages that are written to must belong to one sequence,
+    and the caches may overlap neither each other nor the new tokens (``RuntimeError``, where strides tell).
     No backward pass: called with tensors that require grad (and grad enabled) it raises."""
     if not torch.compiler.is_compiling():
         result = native.na_append(key, value, key_cache, value_cache, page_table, cache_lens, seq_lens, query, frequencies,
