@@ -12,7 +12,9 @@
 //
 // A row's maximum m is fixed at the first columns that it sees and moves only if a later score exceeds it by 2^60 (float16: 2^14),
 // which the row sum of a piece tells; O, the sum and the tile's probabilities so far are then rescaled by the thread itself.  So
-// there is no running maximum, and no thread has to touch O in between.
+// there is no running maximum, and no thread has to touch O in between.  S scale log2(e) - m is one fused operation, so that a
+// score of m's size leaves the rounding of m, half a step, as an exponent: rows with |m| from 2^24 on, where that reaches 1/2, take
+// the rescaling's own arithmetic, which rounds the product first, as m was.
 //
 // Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products, one that walks the CTA's units and
 // hands them to the others (what a unit is takes some hundred instructions and the sequence's lengths, which would stand in
@@ -516,6 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         // =====================================================================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         constexpr float kGrow = BF16 ? 60.f : 14.f;              // headroom of the stored probabilities, as an exponent
+        constexpr float kFar = 16777216.f;                       // 2^24
         constexpr float kGrowSum = BF16 ? 1.152921504606847e18f : 16384.f;     // 2^kGrow: a piece's sum below it has none above it
         const int half = warp >> 2, row = (SPLIT ? 0 : half * kHalfRows) + (warp & 3) * 32 + lane;
         const uint32_t trow = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), scol = trow + 128 * half, ocol = trow + kColO + 128 * half;
@@ -545,8 +548,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             float m = tq >= 0 ? -CUDART_INF_F : 0.f, l = 0.f;    // (rows that do not count hold no tile up)
             // rare: a score far above the maximum.  Move it; rescale O (its products so far are done, see bar_s), the sum and the
             // probabilities of this tile's first `pieces` pieces.
-            auto rescale = [&](bool grow, float over, bool had_tiles, int pieces) {
-                const float f = grow ? fast_exp2(-over) : 1.f;
+            auto rescale = [&](bool grow, float to, bool had_tiles, int pieces) {
+                const float f = grow ? fast_exp2(m - to) : 1.f;
                 tmem_st_wait();
                 if (had_tiles) {
 #pragma unroll 1
@@ -580,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     tmem_st16(scol + 16 * pc, w);
                 }
                 l *= f;
-                if (grow) m += over;
+                if (grow) m = to;                                // (m + (to - m) would round to the larger one's step)
             };
             bool had_tiles = false;
             for (int j = 0; j < n; ++j, ++seq) {
@@ -615,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                         float top = -CUDART_INF_F;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if ((bits >> i) & 1u) top = fmaxf(top, __uint_as_float(s[i]) * by);
+                            if ((bits >> i) & 1u) top = fmaxf(top, __fmul_rn(__uint_as_float(s[i]), by));
                         if (m == -CUDART_INF_F) m = top;
                     }
                 }
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 // registers until the tile's sum has told that none of them outgrew its maximum.
                 bool stored = false;
                 if ((words[0] & words[1] & words[2] & words[3]) == 0xffffffffu && base + kKeys - 1 <= t_least && t_most - base < A.K &&
-                    !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
+                    !__any_sync(0xffffffffu, !(fabsf(m) < kFar))) {
                     uint32_t s[4][32], pk[4][16];                // two pieces ahead: all four at once would spill
                     const uint64_t nb2 = pack2(-m, -m);
                     uint64_t sum0 = 0ull, sum1 = 0ull;
@@ -695,35 +698,37 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             }
                         }
                         const float rs = sum_a + sum_b;
-                        if (__builtin_expect(!__any_sync(0xffffffffu, !(rs <= kGrowSum)), 1)) {
+                        if (__builtin_expect(!__any_sync(0xffffffffu, !(rs <= kGrowSum && fabsf(base_m) < kFar)), 1)) {
                             l += rs;
                             tmem_st16(scol + 32 * hc, pk[0]);    // over columns of this thread's that have been read
                             tmem_st16(scol + 32 * hc + 16, pk[1]);
                             continue;
                         }
-                        // Rare: a score has outgrown the row's maximum (or is not a number).  16 columns at a time, from TMEM again.
-                        auto exponents = [&](int q, uint32_t (&e)[16]) {
+                        // Rare: a score has outgrown the row's maximum (or is not a number), or the maximum is far from zero.  16 columns
+                        // at a time, from TMEM again.
+                        auto exponents = [&](int q, uint32_t (&e)[16], float from) {     // (scaled scores, from = 0)
                             tmem_ld16(scol + 64 * hc + 16 * q, e);
-                            const float by = landed(A.scale_log2), from = m == -CUDART_INF_F ? 0.f : m;
+                            const float by = landed(A.scale_log2);
                             const uint32_t bits = (q < 2 ? lo : hi) >> (16 * (q & 1));
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
-                                e[i] = __float_as_uint((bits >> i) & 1u ? fmaf(__uint_as_float(e[i]), by, -from) : -CUDART_INF_F);
+                                e[i] = __float_as_uint((bits >> i) & 1u ? __fsub_rn(__fmul_rn(__uint_as_float(e[i]), by), from) : -CUDART_INF_F);
                         };
-                        float over = -CUDART_INF_F;
+                        float top = -CUDART_INF_F;
 #pragma unroll 1
                         for (int q = 0; q < 4; ++q) {
                             uint32_t e[16];
-                            exponents(q, e);
+                            exponents(q, e, 0.f);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) over = fmaxf(over, __uint_as_float(e[i]));
+                            for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(e[i]));
                         }
-                        const bool grow = over > kGrow;
-                        if (__any_sync(0xffffffffu, grow)) rescale(grow, over, had_tiles, 2 * hc);
+                        const bool grow = top - base_m > kGrow;
+                        if (__any_sync(0xffffffffu, grow)) rescale(grow, top, had_tiles, 2 * hc);
+                        const float from = m == -CUDART_INF_F ? 0.f : m;
 #pragma unroll 1
                         for (int q = 0; q < 4; ++q) {
                             uint32_t e[16], w8[8];
-                            exponents(q, e);
+                            exponents(q, e, from);
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const float a = fast_exp2(__uint_as_float(e[2 * i])), b = fast_exp2(__uint_as_float(e[2 * i + 1]));
