@@ -169,12 +169,10 @@ struct Piece {
         if (left > 0) {
             column = scratch->column;
             tile = scratch->tile;
-            const int w = tile.n + A.overhead, at = (int)scratch->at;    // less than w * Hkv
-            while (at - off >= w) {
-                off += w;
-                ++h;
-            }
-            off = at - off;
+            const int w = tile.n + A.overhead;
+            long long at = scratch->at;                      // less than w * Hkv, which may pass 31 bits
+            for (; at >= w; at -= w) ++h;
+            off = (int)at;
             if (A.whole && off > 0) advance(A);              // another CTA's
         }
     }
