@@ -122,6 +122,9 @@ struct Call {
         TORCH_CHECK_VALUE(rank >= 1 && rank <= 3 && (int)ks.size() == rank && (int)st.size() == rank &&
                               (int)dil.size() == rank && (int)causal.size() == rank,
                           "natten_b200: tensors of rank ", t.dim(), " do not match the kernel geometry");
+        for (int a = 0; a < rank; ++a)
+            for (const int64_t n : {ks[a], st[a], dil[a]})
+                TORCH_CHECK_VALUE(n > 0 && n <= 2147483647, "natten_b200: kernel size, stride and dilation must be positive, got ", n);
         p = natten_params_t{};
         p.rank = rank;
         p.dtype = dtype_code(t.scalar_type());
@@ -155,6 +158,35 @@ struct Call {
         return shape;
     }
     int64_t slots() const { return (int64_t)p.kernel[0] * p.kernel[1] * p.kernel[2]; }
+
+    // The kernels index every tensor by the geometry of the first one: what does not fit it would be read or written past its end.
+    // [B, *L, heads, last] with the same B and L as the first
+    void fits(const Tensor& t, int64_t heads, int64_t last, const char* name) const
+    {
+        bool ok = t.dim() == rank + 3 && t.size(0) == p.batch && t.size(rank + 1) == heads && t.size(rank + 2) == last;
+        for (int a = 0; a < rank && ok; ++a) ok = t.size(1 + a) == p.extent[a];
+        TORCH_CHECK_VALUE(ok, "natten_b200: ", name, " of shape ", t.sizes(), " does not fit the others");
+    }
+    // an output's shape
+    void fits_out(const Tensor& t, int64_t last, const char* name)
+    {
+        TORCH_CHECK_VALUE(t.sizes() == out_shape(p.heads_q, last), "natten_b200: ", name, " of shape ", t.sizes(), " does not fit the others");
+    }
+    void fits_extra(const Tensor& ek, const Tensor& ev) const
+    {
+        if (!ek.defined() && !ev.defined()) return;
+        const bool ok = ek.defined() && ev.defined() && ek.dim() == 4 && ev.dim() == 4 && ek.size(0) == p.batch && ev.size(0) == p.batch &&
+                        ek.size(1) == ev.size(1) && ek.size(2) == p.heads_kv && ev.size(2) == p.heads_kv && ek.size(3) == p.dim &&
+                        ev.size(3) == p.dim_v;
+        TORCH_CHECK_VALUE(ok, "natten_b200: additional keys and values do not fit the others");
+    }
+    // bias of shape [heads, 2 kernel - 1 ...]
+    void fits_bias(IntArrayRef s) const
+    {
+        bool ok = (int)s.size() == rank + 1 && s[0] == p.heads_q;
+        for (int a = 0; a < rank && ok; ++a) ok = s[1 + a] == 2 * (int64_t)p.kernel[a] - 1;
+        TORCH_CHECK_VALUE(ok, "natten_b200: a bias of shape ", s, " does not fit the kernel");
+    }
 };
 
 Tensor fresh(IntArrayRef shape, at::ScalarType dtype, const Tensor& like)
@@ -173,6 +205,8 @@ Tensor as(const Tensor& t, at::ScalarType dtype)
 void set_extents(natten_params_t& p, const OptTensor& extents, const Tensor& q, Tensor& held)
 {
     if (!extents || !extents->defined()) return;
+    TORCH_CHECK_VALUE(extents->numel() == (int64_t)p.batch * p.rank, "natten_b200: extents of shape ", extents->sizes(), " for a batch of ",
+                      p.batch);
     held = extents->to(q.device(), at::kInt).reshape({-1, p.rank}).contiguous();
     p.extents = held.const_data_ptr<int32_t>();
 }
@@ -190,9 +224,12 @@ std::tuple<Tensor, Tensor> fused_cuda(const Tensor& q_in, const Tensor& k_in, co
                                       IntArrayRef dil, Bools causal, double scale)
 {
     Tensor ek = ek_in.value_or(Tensor()), ev = ev_in.value_or(Tensor());
+    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), v_in.size(-1), ks, st, dil, causal);
+    c.fits(k_in, c.p.heads_kv, c.p.dim, "key");
+    c.fits(v_in, c.p.heads_kv, c.p.dim_v, "value");
+    c.fits_extra(ek, ev);
     require_cuda({&q_in, &k_in, &v_in, &ek, &ev}, q_in);
     same_dtype(q_in, {&k_in, &v_in, &ek, &ev});
-    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), v_in.size(-1), ks, st, dil, causal);
     const Tensor q = strided_input(q_in, c.rank, c.p.q_stride), k = strided_input(k_in, c.rank, c.p.k_stride),
                  v = strided_input(v_in, c.rank, c.p.v_stride);
     if (ek.defined()) {
@@ -218,14 +255,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> fused_bwd_cuda(
     IntArrayRef ks, IntArrayRef st, IntArrayRef dil, Bools causal, double scale)
 {
     Tensor ek = ek_in.value_or(Tensor()), ev = ev_in.value_or(Tensor()), dlse = dlse_in.value_or(Tensor());
+    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), v_in.size(-1), ks, st, dil, causal);
+    c.fits(k_in, c.p.heads_kv, c.p.dim, "key");
+    c.fits(v_in, c.p.heads_kv, c.p.dim_v, "value");
+    c.fits_extra(ek, ev);
+    c.fits_out(out_in, c.p.dim_v, "output");
+    c.fits_out(dout_in, c.p.dim_v, "gradient");
+    c.fits_out(lse_in, -1, "log-sum-exp");
+    if (dlse.defined()) c.fits_out(dlse, -1, "gradient of the log-sum-exp");
     require_cuda({&q_in, &k_in, &v_in, &ek, &ev, &out_in, &lse_in, &dout_in, &dlse}, q_in);
     same_dtype(q_in, {&k_in, &v_in, &ek, &ev, &out_in});
-    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), v_in.size(-1), ks, st, dil, causal);
     const Tensor q = strided_input(q_in, c.rank, c.p.q_stride), k = strided_input(k_in, c.rank, c.p.k_stride),
                  v = strided_input(v_in, c.rank, c.p.v_stride);
     c.scale(scale);
     const c10::cuda::CUDAGuard guard(q.device());
-    const Tensor out = out_in.contiguous(), lse = lse_in.contiguous(), dout = as(dout_in, q.scalar_type());
+    const Tensor out = out_in.contiguous(), lse = as(lse_in, acc_type(q.scalar_type())), dout = as(dout_in, q.scalar_type());
     if (dlse.defined()) dlse = as(dlse, lse.scalar_type());
     Tensor dek, dev;
     if (ek.defined()) {
@@ -256,9 +300,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> fused_bwd_cuda(
 Tensor qk_cuda(const Tensor& q_in, const Tensor& k_in, IntArrayRef ks, IntArrayRef dil, IntArrayRef st, Bools causal,
                std::optional<double> scale)
 {
+    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), q_in.size(-1), ks, st, dil, causal);
+    c.fits(k_in, c.p.heads_kv, c.p.dim, "key");
     require_cuda({&q_in, &k_in}, q_in);
     same_dtype(q_in, {&k_in});
-    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), q_in.size(-1), ks, st, dil, causal);
     const Tensor q = strided_input(q_in, c.rank, c.p.q_stride), k = strided_input(k_in, c.rank, c.p.k_stride);
     std::copy(c.p.k_stride, c.p.k_stride + 3, c.p.v_stride);
     if (scale) c.scale(*scale);
@@ -272,9 +317,11 @@ Tensor qk_cuda(const Tensor& q_in, const Tensor& k_in, IntArrayRef ks, IntArrayR
 std::tuple<Tensor, Tensor> qk_bwd_cuda(const Tensor& dlogits_in, const Tensor& q_in, const Tensor& k_in, IntArrayRef ks,
                                        IntArrayRef dil, IntArrayRef st, Bools causal, std::optional<double> scale)
 {
+    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), q_in.size(-1), ks, st, dil, causal);
+    c.fits(k_in, c.p.heads_kv, c.p.dim, "key");
+    c.fits_out(dlogits_in, c.slots(), "gradient");
     require_cuda({&q_in, &k_in, &dlogits_in}, q_in);
     same_dtype(q_in, {&k_in});
-    Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), q_in.size(-1), ks, st, dil, causal);
     const Tensor q = strided_input(q_in, c.rank, c.p.q_stride), k = strided_input(k_in, c.rank, c.p.k_stride);
     std::copy(c.p.k_stride, c.p.k_stride + 3, c.p.v_stride);
     if (scale) c.scale(*scale);
@@ -295,10 +342,12 @@ struct Unit {                                // unit stride, no causal axis: wha
 Tensor qk_rpb_cuda(const Tensor& q_in, const Tensor& k_in, const Tensor& rpb_in, IntArrayRef ks, IntArrayRef dil,
                    std::optional<double> scale)
 {
-    require_cuda({&q_in, &k_in, &rpb_in}, q_in);
-    same_dtype(q_in, {&k_in});
     const Unit u(ks.size());
     Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), q_in.size(-1), ks, u.ones, dil, u.no);
+    c.fits(k_in, c.p.heads_kv, c.p.dim, "key");
+    c.fits_bias(rpb_in.sizes());
+    require_cuda({&q_in, &k_in, &rpb_in}, q_in);
+    same_dtype(q_in, {&k_in});
     const Tensor q = strided_input(q_in, c.rank, c.p.q_stride), k = strided_input(k_in, c.rank, c.p.k_stride);
     std::copy(c.p.k_stride, c.p.k_stride + 3, c.p.v_stride);
     if (scale) c.scale(*scale);
@@ -314,10 +363,13 @@ std::tuple<Tensor, Tensor, Tensor> qk_rpb_bwd_cuda(const Tensor& dlogits_in, con
                                                    IntArrayRef rpb_shape, IntArrayRef ks, IntArrayRef dil,
                                                    std::optional<double> scale)
 {
-    require_cuda({&q_in, &k_in, &dlogits_in}, q_in);
-    same_dtype(q_in, {&k_in});
     const Unit u(ks.size());
     Call c(q_in, q_in.size(-2), k_in.size(-2), q_in.size(-1), q_in.size(-1), ks, u.ones, dil, u.no);
+    c.fits(k_in, c.p.heads_kv, c.p.dim, "key");
+    c.fits_bias(rpb_shape);
+    c.fits_out(dlogits_in, c.slots(), "gradient");
+    require_cuda({&q_in, &k_in, &dlogits_in}, q_in);
+    same_dtype(q_in, {&k_in});
     const Tensor q = strided_input(q_in, c.rank, c.p.q_stride), k = strided_input(k_in, c.rank, c.p.k_stride);
     std::copy(c.p.k_stride, c.p.k_stride + 3, c.p.v_stride);
     if (scale) c.scale(*scale);
@@ -333,8 +385,9 @@ std::tuple<Tensor, Tensor, Tensor> qk_rpb_bwd_cuda(const Tensor& dlogits_in, con
 
 Tensor av_cuda(const Tensor& attn_in, const Tensor& v_in, IntArrayRef ks, IntArrayRef dil, IntArrayRef st, Bools causal)
 {
-    require_cuda({&v_in, &attn_in}, v_in);
     Call c(v_in, attn_in.size(-2), v_in.size(-2), v_in.size(-1), v_in.size(-1), ks, st, dil, causal);
+    c.fits_out(attn_in, c.slots(), "attention");
+    require_cuda({&v_in, &attn_in}, v_in);
     const Tensor v = strided_input(v_in, c.rank, c.p.v_stride);
     std::copy(c.p.v_stride, c.p.v_stride + 3, c.p.q_stride);
     std::copy(c.p.v_stride, c.p.v_stride + 3, c.p.k_stride);
@@ -351,8 +404,10 @@ Tensor av_cuda(const Tensor& attn_in, const Tensor& v_in, IntArrayRef ks, IntArr
 std::tuple<Tensor, Tensor> av_bwd_cuda(const Tensor& dout_in, const Tensor& attn_in, const Tensor& v_in, IntArrayRef ks,
                                        IntArrayRef dil, IntArrayRef st, Bools causal)
 {
-    require_cuda({&v_in, &attn_in, &dout_in}, v_in);
     Call c(v_in, attn_in.size(-2), v_in.size(-2), v_in.size(-1), v_in.size(-1), ks, st, dil, causal);
+    c.fits_out(attn_in, c.slots(), "attention");
+    c.fits_out(dout_in, c.p.dim_v, "gradient");
+    require_cuda({&v_in, &attn_in, &dout_in}, v_in);
     const Tensor v = strided_input(v_in, c.rank, c.p.v_stride);
     std::copy(c.p.v_stride, c.p.v_stride + 3, c.p.q_stride);
     std::copy(c.p.v_stride, c.p.v_stride + 3, c.p.k_stride);
