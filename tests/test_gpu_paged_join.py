@@ -30,6 +30,19 @@ def _check(q, k_cache, v_cache, table, lens, kernel=None):
     return out, lse
 
 
+@pytest.mark.parametrize("form", [
+    (F16, 1, 4, 1, 64), (F16, 3, 8, 2, 128), (BF16, 1, 4, 1, 256), (F16, 2, 4, 2, 160), (BF16, 5, 2, 1, 136),      # warps
+    (BF16, 40, 2, 1, 128), (F16, 40, 4, 2, 64), (F16, 70, 8, 2, 64), (BF16, 100, 8, 2, 128),                      # tcgen05
+    (F32, 2, 2, 1, 200), (F32, 2, 4, 2, 6), (F16, 1, 2, 1, 5), (BF16, 3, 2, 1, 130), (F32, 17, 2, 2, 129)], ids=str)
+@pytest.mark.parametrize("kernel", [None, 2049])
+def test_types_and_head_dims(form, kernel):
+    """Head dims above 128, not a multiple of 4, every type, split keys."""
+    problem = _problem(*form)
+    a = _check(*problem, kernel)
+    b = _check(*problem, kernel)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 @pytest.mark.parametrize("form", FORMS, ids=str)
 def test_a_query_that_is_not_a_number_shows(form):
     q, *cache = _problem(*form)
