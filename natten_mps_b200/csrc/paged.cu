@@ -48,9 +48,9 @@ template <typename T, int ROWS, int DC> __global__ void __launch_bounds__(kJoinT
         bool bad = false;
         if (real)
             for (int i = lane; i < parts; i += 32) {
-                const float2 ml = slot_sums(A, slot(i))[row];
-                bad = bad || ml.x != ml.x || ml.y != ml.y;               // scores that are not numbers leave no maximum, but such a sum
-                top = fmaxf(top, ml.x);
+                const float m = slot_sums(A, slot(i))[row].x;
+                bad = bad || m != m;
+                top = fmaxf(top, m);
             }
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -88,7 +88,7 @@ template <typename T, int ROWS, int DC> __global__ void __launch_bounds__(kJoinT
 #pragma unroll
                 for (int k = 0; k < kAtOnce; ++k) {
                     const float f = exp2f(ml[k].x - base);
-                    if (ml[k].y == 0.f) continue;                        // a part that saw nothing
+                    if (ml[k].y == 0.f) continue;                        // a part that saw nothing (NaN scores leave m = -inf, l = NaN)
                     total = fmaf(f, ml[k].y, total);
 #pragma unroll
                     for (int d = 0; d < DC; ++d) {
