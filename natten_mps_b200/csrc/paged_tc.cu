@@ -525,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         float2* sums = reinterpret_cast<float2*>(smem + C::kOffSums);
         bool ok = !gave_up(abort_flag);
         unsigned mine = 0, seq = 0, units = 0, exchanges = 0;    // tiles of this half, tiles of the CTA, units of this half
+        bool skipped = false;                                    // the last unit, without a look at its tiles
         const uint64_t sc2 = pack2(A.scale_log2, A.scale_log2);
         for (unsigned walked = 0; ok;) {
             const Unit p = next_unit(walked);
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             const bool active = SPLIT ? half == 0 || n > 1 : half == 0 || x.rows > kHalfRows;
             if (!active) {
                 seq += n;
+                skipped = true;
                 continue;
             }
             long long index = -1;
@@ -590,10 +592,11 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                 if (SPLIT && (j & 1) != half) continue;
                 const int base = x.base + (p.x0 + j) * kKeys;
                 const unsigned w = seq % kWordSlots;
-                // A half that took no part in the units before may be here long before this tile's words are: its barrier would be
-                // two phases behind, and one bit of phase cannot tell that from done.  So the first tile of a unit waits for its
-                // scores first (they are issued behind the words); from then on the words of tile seq - 16 are known to be past.
-                if (!had_tiles) ok = ok && mbar_wait(bar_s + 8 * half, mine & 1, abort_flag, P.wait_budget);
+                // A half that left units out may be here long before this tile's words are: their barrier could be two phases
+                // behind, which one bit of phase cannot tell from done.  So it waits for the tile's scores first, which are issued
+                // behind the words.  With the tile before seen, the words of tile seq - 16 are known to be past.
+                if (skipped) ok = ok && mbar_wait(bar_s + 8 * half, mine & 1, abort_flag, P.wait_budget);
+                skipped = false;
                 ok = ok && mbar_wait(bar_words + 8 * w, (seq / kWordSlots) & 1, abort_flag, P.wait_budget);
                 const volatile uint32_t* there_words = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffWords) + 4 * w;
                 const uint32_t words[4] = {there_words[0], there_words[1], there_words[2], there_words[3]};
