@@ -548,6 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             const int t_least = __reduce_min_sync(0xffffffffu, live ? tq : 0x7fffffff), t_most = __reduce_max_sync(0xffffffffu, live ? tq : -1);
             if (!live) tq = -1;
             float m = tq >= 0 ? -CUDART_INF_F : 0.f, l = 0.f;    // (rows that do not count hold no tile up)
+            float limit = kGrowSum;                              // of a piece's sum; rows far from zero always go past it
             // rare: a score far above the maximum.  Move it; rescale O (its products so far are done, see bar_s), the sum and the
             // probabilities of this tile's first `pieces` pieces.
             auto rescale = [&](bool grow, float to, bool had_tiles, int pieces) {
@@ -585,7 +586,10 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     tmem_st16(scol + 16 * pc, w);
                 }
                 l *= f;
-                if (grow) m = to;                                // (m + (to - m) would round to the larger one's step)
+                if (grow) {
+                    m = to;                                      // (m + (to - m) would round to the larger one's step)
+                    limit = fabsf(to) < kFar ? kGrowSum : -1.f;
+                }
             };
             bool had_tiles = false;
             for (int j = 0; j < n; ++j, ++seq) {
@@ -622,14 +626,17 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if ((bits >> i) & 1u) top = fmaxf(top, __fmul_rn(__uint_as_float(s[i]), by));
-                        if (m == -CUDART_INF_F) m = top;
+                        if (m == -CUDART_INF_F) {
+                            m = top;
+                            if (fabsf(top) >= kFar && top != -CUDART_INF_F) limit = -1.f;
+                        }
                     }
                 }
                 // A tile that every row of the warp sees all of (most of a long context): no masks, and the probabilities stay in
                 // registers until the tile's sum has told that none of them outgrew its maximum.
                 bool stored = false;
                 if ((words[0] & words[1] & words[2] & words[3]) == 0xffffffffu && base + kKeys - 1 <= t_least && t_most - base < A.K &&
-                    !__any_sync(0xffffffffu, !(fabsf(m) < kFar))) {
+                    !__any_sync(0xffffffffu, m == -CUDART_INF_F)) {
                     uint32_t s[4][32], pk[4][16];                // two pieces ahead: all four at once would spill
                     const uint64_t nb2 = pack2(-m, -m);
                     uint64_t sum0 = 0ull, sum1 = 0ull;
@@ -660,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     }
                     sum0 = add2(sum0, sum1);
                     const float rs = lo_of(sum0) + hi_of(sum0);
-                    if (!__any_sync(0xffffffffu, !(rs <= kGrowSum))) {
+                    if (!__any_sync(0xffffffffu, !(rs <= limit))) {
                         l += rs;
                         stored = true;
 #pragma unroll
@@ -701,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             }
                         }
                         const float rs = sum_a + sum_b;
-                        if (__builtin_expect(!__any_sync(0xffffffffu, !(rs <= kGrowSum && fabsf(base_m) < kFar)), 1)) {
+                        if (__builtin_expect(!__any_sync(0xffffffffu, !(rs <= limit)), 1)) {
                             l += rs;
                             tmem_st16(scol + 32 * hc, pk[0]);    // over columns of this thread's that have been read
                             tmem_st16(scol + 32 * hc + 16, pk[1]);
