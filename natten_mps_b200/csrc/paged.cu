@@ -244,7 +244,7 @@ int choose(const natten_paged_params_t* p, Chosen& c, const void* q, const void*
     const bool simt = (p->flags & NATTEN_FLAG_FORCE_SIMT) != 0;
     Shape shape;
     Args general = A;
-    if (!general_shape(p->dtype, general, c.aligned, shape) || !divide(general, shape)) return NATTEN_E_UNSUPPORTED;
+    if (!general_shape(p->dtype, general, shape) || !divide(general, shape)) return NATTEN_E_UNSUPPORTED;
     c.family = Family::kGeneral;
     c.workspace = workspace_of(general);
     const bool tc = !simt && tc_shape(p->dtype, A, p->dim % 8 == 0, shape);

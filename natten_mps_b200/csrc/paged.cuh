@@ -244,11 +244,11 @@ __device__ __forceinline__ bool locate(const Args& A, const Tile& x, int t, int&
     return page >= 0 && page < A.pages;
 }
 
-// Host side.  A kernel family says which tiles it would use (false: it does not cover the call); `plan` divides the call by
-// them.  `aligned`: every row of q and of the caches starts on a 16-byte boundary.
+// Host side.  A kernel family says which tiles it would use (false: it does not cover the call); `divide` (paged.cu) divides the
+// call by them.  `aligned`: every row of q and of the caches starts on a 16-byte boundary, or could.
 // most: key tiles up to which a unit is not shared
 struct Shape { int M, keys, overhead, least, most, ctas; };
-bool general_shape(int dtype, const Args& A, bool aligned, Shape& shape);
+bool general_shape(int dtype, const Args& A, Shape& shape);
 int general_run(int dtype, const Args& A, bool aligned, cudaStream_t s);
 bool warp_shape(int dtype, const Args& A, bool aligned, int warps, Shape& shape);
 int warp_run(int dtype, const Args& A, int warps, cudaStream_t s);
@@ -264,7 +264,4 @@ __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontro
 
 void note_path(int path);        // what natten_last_path reports
 
-namespace paged {
-
-} // namespace paged
 } // namespace natten

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const __grid_constant
 
 } // namespace
 
-bool general_shape(int dtype, const Args& A, bool, Shape& shape)
+bool general_shape(int dtype, const Args& A, Shape& shape)
 {
     if (dtype != NATTEN_F32 && dtype != NATTEN_F16 && dtype != NATTEN_BF16) return false;
     shape = {kRows, kKeys, 1, 1, 16, 3 * sm_count()};
