@@ -25,9 +25,14 @@
 // into the same swizzled layout; a row that is not there is zero, whatever its slot holds.  Row-wise copies of every tile would
 // take 3750 cycles a tile, twice what the products need.  The queries come by TMA where a group's heads divide the tile, too.
 //
-// Measured on one B200, bf16, 16 heads of 128 on 4: chunks of 2048 tokens over caches of 16384, batch 2, 441 - 454 us at 1.97 GHz
-// (1120 - 1140 TFLOP/s), 514 us back to back, where the power cap holds the clock at 1.63 GHz; prompts of 8191 through a window
-// of 255, batch 2, 91 us.  The tensor products of a tile are 2048 cycles for both halves, the exponentials 1024 a half on the special-
+// P is rounded to the tensors' type, since the product takes one type: half a step of each weight, where the output itself is rounded
+// by as much.  The row sum adds the weights as they were.  Against 64 bits the outputs are off by 0.0022 - 0.0024 of their size in
+// bfloat16 and 0.00027 in float16, where the output's rounding alone leaves 0.0017 and 0.00021; a second product with what the
+// rounding cut off would bring that back for half as many tensor products again.
+//
+// Measured on one B200, bf16, 16 heads of 128 on 4: chunks of 2048 tokens over caches of 16384, batch 2, 455 - 464 us at 1.97 GHz
+// with pauses (1110 - 1130 TFLOP/s), 519 - 528 us back to back (980 - 990), where the power cap holds the clock at 1.6 GHz; prompts of
+// 8191 through a window of 255, batch 2, 91 - 93 us.  The tensor products of a tile are 2048 cycles for both halves, the exponentials 1024 a half on the special-
 // function unit; with time stamps in the kernel a tile took 3600 cycles, in which a half spent about 1600 on its exponentials and
 // waited about 1100 for its products, behind the other half's.  Short units of a window have masked tiles and outputs instead.
 //
@@ -892,7 +897,8 @@ bool tc_shape(int dtype, const Args& A, bool aligned, Shape& shape)
     if ((dtype != NATTEN_F16 && dtype != NATTEN_BF16) || !aligned || (A.D != 64 && A.D != 128)) return false;
     const long long rows = ((long long)A.L + A.dil - 1) / A.dil * A.G;
     // 36 rows a unit over a context of 8192 (16 sequences): 76 us here, 149 on the other kernel; 64 rows over 8192 (8 sequences) 52 | 84.
-    // A short context goes the other way (64 rows of 64 channels over 1024, 32 sequences: 32 | 25), but its length is on the device.
+    // A short context goes the other way (64 rows of 64 channels over 1024, 32 sequences: 32 | 25).  Its length is on the device; of the
+    // bound that the host has, window and table (`divide`), this rule makes no use.
     if (rows <= 32) return false;
     shape = {rows > kHalfRows ? 2 * kHalfRows : kHalfRows, kKeys, 1, 2, 8, sm_count()};
     return true;

@@ -7,11 +7,15 @@
 // its own maximum, and accumulates all channels of its weighted sum in registers.  Nothing in the loop waits for another warp.
 // At the end of the unit the warps' partial results are joined through shared memory.
 //
-// Measured on one B200, bf16, 16 heads of 128 on 4: one token for each of 64 sequences of 2048 - 16384 tokens 192 us (6.3 TB/s with the
-// join, 96 % of a copy); 8 sequences through a window of 255 7.7 us, where lengths, page table, first keys and the join of the warps
+// Measured on one B200, bf16, 16 heads of 128 on 4: one token for each of 64 sequences of 2048 - 16384 tokens 191 us in a graph,
+// 192 - 205 us over ten runs with other inputs in between (5.9 - 6.4 TB/s with the join, 90 - 97 % of a copy); 8 sequences through a window of 255 7.7 us, where lengths, page table, first keys and the join of the warps
 // follow each other.  Eight warps a CTA or four and two CTAs an SM: with more short units than SMs two CTAs fill each other's
 // beginnings and ends (128 sequences, window 512: 31 us against 37.5), with fewer the unit's keys want all warps (32 sequences of
 // 512: 10.4 against 14.3).
+//
+// Weights are rounded to the tensors' type for their product with the values, which takes one type: half a step of each, as much as
+// the rounding of the output; the row sum adds them as they were.  Against 64 bits the outputs are off by 0.0020 - 0.0022 of their size
+// in bfloat16 and 0.00027 in float16, where the output's rounding alone leaves 0.0017 and 0.00021.
 //
 // A key that no row of the unit sees (behind the last query, in front of the first window, on a page that is not there) is not
 // fetched: its line of shared memory is zero.  One that some rows see and others do not is multiplied by a weight of zero in those,
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(Cfg<DP, MT, NW>::kThreads, Cfg<DP, MT, NW>::kP
                     for (int n = 0; n < NT; ++n) {
                         const float a = fast_exp2(sc[m][n][2 * i] - base_m), b = fast_exp2(sc[m][n][2 * i + 1] - base_m);
                         total[m][i] += a + b;
-                        w[m][n][i] = cvt_pack<BF16>(a, b);       // weights are at most 1: half a step of the type (see the header)
+                        w[m][n][i] = cvt_pack<BF16>(a, b);       // weights are at most 1: half a step of the type
                     }
                 }
 #pragma unroll

@@ -150,7 +150,8 @@ class NeighborhoodAttention1D(_NeighborhoodAttention):
     """1-D module; ``forward(x [B, L, C], seq_lens=None)``.
 
     ``rotary_dim > 0`` turns the first ``rotary_dim`` channels of every query and key head by their positions
-    (``rotary_base``, ``rotary_interleaved``; ``rotary_scaling``: keyword arguments of ``rotary_frequencies``).
+    (``rotary_base``, ``rotary_interleaved``; ``rotary_scaling``: keyword arguments of ``rotary_frequencies``).  Their
+    frequencies are copied to a device at the first call there, which therefore cannot be inside a graph capture.
 
     ``forward(x, cache=layer)`` serves a decoder: ``x [B, L, C]`` are new tokens behind those that ``layer`` (a
     ``PagedCache.layer``, extended for them) holds; their keys and values are appended, and they attend to the cache
