@@ -13,7 +13,7 @@
 // A row's maximum m is fixed at the first columns that it sees and moves only if a later score exceeds it by 2^60 (float16: 2^14),
 // which the row sum of a piece tells; O, the sum and the tile's probabilities so far are then rescaled by the thread itself.  So
 // there is no running maximum, and no thread has to touch O in between.  S scale log2(e) - m is one fused operation, so that a
-// score of m's size leaves the rounding of m, half a step, as an exponent: rows with |m| from 2^24 on, where that reaches 1/2, take
+// score of m's size leaves the rounding of m, half a step, as an exponent: rows with |m| from 2^24 on, where that passes 1/2, take
 // the rescaling's own arithmetic, which rounds the product first, as m was.
 //
 // Sixteen warps: two warpgroups of softmax, one that loads, one warp that issues the products, one that walks the CTA's units and
